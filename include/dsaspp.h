@@ -552,6 +552,67 @@ typedef struct dsaspp_prep_desc {
 int dsaspp_preprocess(const dsaspp_prep_desc* d, dsaspp_stream_t stream);
 
 /* ------------------------------------------------------------------------------------
+ * Class scores: log probability of a given label, entropy and the most probable classes of every row (a pixel, a token) of a
+ * tensor of logits, and their gradient.  It sits next to dsaspp_upsample8_argmax / _ce: the reference only has the arg-max and
+ * the mean loss of the same logits (graph_seg_test.py:62, graph_seg_main.py:238).
+ *   log_p[c] = z[c] - logsumexp(z),  p = exp(log_p)
+ *   logp = log_p[label]; 0 for a row without a label: label == ignore_index or outside [0, n_class)
+ *   entropy = -sum p log_p, top_class / top_logp: the top_k largest logits, descending, the lowest class first among equal ones
+ * Classes at -inf are masked out: p = 0, never an alternative; alternatives a row does not have are -1 with log probability -inf.
+ * A row with nothing but -inf: logp -inf (if labelled), entropy 0, gradient 0.  A row with a NaN or +inf: logp (if labelled), entropy
+ * and top_logp NaN, top_class -1.  The gradient of a row whose upstream gradients are all 0 is 0 whatever its logits hold.
+ * Backward, a = g_logp (0 without a label), b = g_entropy, t_j = g_top[j] (0 at -1), A = a + sum t_j:
+ *   dz[c] = a [c == label] + sum_j t_j [c == top_class[j]] - p[c] A - b p[c] (log_p[c] + entropy)
+ *
+ * Rows are numbered (i0, i1, i2) row-major over [d0][d1][d2]; logits of row (i0, i1, i2), class c at
+ * logits[i0*s0 + i1*s1 + i2*s2 + c*sc] (strides in elements, >= 0).  labels, logp and entropy are dense [rows];
+ * top_logp and top_class are [d0][top_k][d1][d2].  dlogits is dense: [rows][n_class] when sc == 1, else [d0][n_class][d1][d2].
+ * Arithmetic is fp32 on logits of any dtype; dlogits has the logits' dtype (0 = bf16, 1 = fp32, 2 = fp16), rounded once. */
+#define DSASPP_SCORES_MAX_TOP 8
+typedef struct dsaspp_scores_desc {
+    int32_t dtype, n_class, top_k;
+    int64_t d0, d1, d2;
+    int64_t s0, s1, s2, sc;
+    const void* logits;
+    const int64_t* labels;    /* may be NULL: then logp must be NULL too */
+    int64_t ignore_index;
+    float* logp;              /* outputs of the forward call, each may be NULL; inputs of the backward call: stats, entropy */
+    float* entropy;           /* (only when g_entropy is given) and top_class (only when g_top is given) */
+    float* stats;             /* [rows][2] for the backward call: largest logit, log of the sum of exponentials relative to it */
+    float* top_logp; int64_t* top_class;
+    /* backward: upstream gradients, each may be NULL (counts as 0); *_one != 0: one value for all rows / entries */
+    const float* g_logp; const float* g_entropy; const float* g_top;
+    int32_t g_logp_one, g_entropy_one, g_top_one;
+    void* dlogits;
+} dsaspp_scores_desc;
+int dsaspp_scores_fwd(const dsaspp_scores_desc* d, dsaspp_stream_t stream);
+int dsaspp_scores_bwd(const dsaspp_scores_desc* d, dsaspp_stream_t stream);
+
+/* The same on logits at 1/8 resolution, with the bilinear x8 upsample (align_corners=False) fused in: the full-resolution logits
+ * are never written.  z = hy*r0 + ly*r1, r_i = hx*L[yi][x0] + lx*L[yi][x1], every product and sum rounded to fp32 by itself, so the
+ * order of the classes is that of those values to the bit.  n_class <= 32.  Logits of image n, pixel (y, x), class c at
+ * logits[n*sn + y*sy + x*sx + c*sc]; labels, logp, entropy [n_img][8h][8w]; top_* [n_img][top_k][8h][8w]; upstream gradients
+ * likewise.  Backward reads logits, labels and (with g_top) top_class; dlogits at dlogits[n*gn + y*gy + x*gx + c*gc], dtype g_dtype;
+ * ws: dsaspp_scores8_workspace floats, contents need not be initialised. */
+typedef struct dsaspp_scores8_desc {
+    int32_t n_img, h, w, n_class, top_k;
+    int32_t dtype, g_dtype;
+    int64_t sn, sy, sx, sc;
+    const void* logits;
+    const int64_t* labels;
+    int64_t ignore_index;
+    float* logp; float* entropy; float* top_logp; int64_t* top_class;
+    const float* g_logp; const float* g_entropy; const float* g_top;
+    int32_t g_logp_one, g_entropy_one, g_top_one;
+    void* dlogits;
+    int64_t gn, gy, gx, gc;
+    float* ws; int64_t ws_len;
+} dsaspp_scores8_desc;
+int64_t dsaspp_scores8_workspace(const dsaspp_scores8_desc* d); /* floats for the backward call; -1 on a bad descriptor */
+int dsaspp_scores8_fwd(const dsaspp_scores8_desc* d, dsaspp_stream_t stream);
+int dsaspp_scores8_bwd(const dsaspp_scores8_desc* d, dsaspp_stream_t stream);
+
+/* ------------------------------------------------------------------------------------
  * Parameter-side kernels over the flat parameter arena (adjacent to the path:
  * torch.optim.Adam(weight_decay) + poly learning rate, reference graph_seg_main.py:186,241-245).
  */
@@ -566,6 +627,50 @@ typedef struct dsaspp_adam_desc {
     float grad_scale;         /* multiply g first (e.g. 1/world_size) */
 } dsaspp_adam_desc;
 int dsaspp_adam_step(const dsaspp_adam_desc* d, dsaspp_stream_t stream);
+
+/* ------------------------------------------------------------------------------------
+ * Global gradient norm over many tensors, clipping by it, and the Adam update with the clip coefficient applied on the fly
+ * (what torch.nn.utils.clip_grad_norm_ + torch.optim.Adam do between backward and the next step).
+ *   norm = scale * sqrt(sum over all ranges of g^2)   (norm_type 2)      scale * max |g|   (norm_type 0)
+ *   coef = min(1, max_norm / (norm + 1e-6))           a NaN norm gives a NaN coefficient
+ * The gradients are a HOST array of dense device ranges; it is read during the call only and may be freed after it.  A range
+ * needs no more alignment than its element type.  Sums are fp64 (the square of an fp32 value is exact there and cannot overflow) and
+ * taken in an order that depends on the list of sizes alone, so equal lists give equal bits.
+ *   1. dsaspp_grad_norm_partials: one fp64 partial per block into ws (dsaspp_grad_norm_workspace doubles, contents need not be
+ *      initialised).  n_ranges == 0 is allowed: the norm is 0.
+ *   2. dsaspp_grad_norm_finish: norm[0] from the partials; or
+ *      dsaspp_clip_scale: every range times coef in place, rounded once to its type (ranges are left untouched where coef is 1),
+ *      norm[0] too; or dsaspp_adam_step_clipped: the Adam update with g * scale * coef; g itself is not written.
+ * The three read the partials and nothing but the partials: call 1 with the same ranges first, on the same stream.
+ * dtype of a range: 0 = bf16, 1 = fp32, 2 = fp16. */
+typedef struct dsaspp_grad_range {
+    void* p;
+    int64_t n;                /* elements, > 0 */
+    int32_t dtype, pad;
+} dsaspp_grad_range;
+typedef struct dsaspp_clip_desc {
+    const dsaspp_grad_range* ranges; /* host */
+    int32_t n_ranges;
+    int32_t norm_type;        /* 2 = Euclidean, 0 = largest magnitude */
+    float scale;              /* the gradients count as scale * g (> 0); dsaspp_clip_scale takes 1 only */
+    float max_norm;           /* >= 0, may be +inf */
+    double* ws; int64_t ws_len; /* device, in doubles */
+    float* norm;              /* device, 1 float */
+} dsaspp_clip_desc;
+int64_t dsaspp_grad_norm_workspace(const dsaspp_clip_desc* d); /* doubles; -1 on a bad descriptor */
+int dsaspp_grad_norm_partials(const dsaspp_clip_desc* d, dsaspp_stream_t stream);
+int dsaspp_grad_norm_finish(const dsaspp_clip_desc* d, dsaspp_stream_t stream);
+int dsaspp_clip_scale(const dsaspp_clip_desc* d, dsaspp_stream_t stream);
+/* The update of dsaspp_adam_step with g * c->scale * coef, on any n > 0 elements with no more alignment than their type.  The factors
+ * come in double, as an optimizer's host code holds them: 1 - beta2 of a beta2 rounded to fp32 is 1.3e-5 off at 0.999. */
+typedef struct dsaspp_adam_clip_desc {
+    int64_t n;
+    float* p; const float* g; float* m; float* v;
+    void* w16;                /* bf16 copy of p, may be NULL */
+    double lr, beta1, beta2, eps, weight_decay;
+    int64_t step;             /* 1-based */
+} dsaspp_adam_clip_desc;
+int dsaspp_adam_step_clipped(const dsaspp_adam_clip_desc* a, const dsaspp_clip_desc* c, dsaspp_stream_t stream);
 
 /* fp32 -> bf16 cast of the flat arena */
 int dsaspp_cast_bf16(const float* src, void* dst, int64_t n, dsaspp_stream_t stream);

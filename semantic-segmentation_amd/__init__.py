@@ -6,5 +6,6 @@ statement; ``denseASPP.py`` at the repository root loads it under the module nam
 """
 from .dense_aspp import DenseASPP  # noqa: F401
 from .spec import NetSpec  # noqa: F401
+from .scores import Scores, label_scores  # noqa: F401
 
-__all__ = ['DenseASPP', 'NetSpec']
+__all__ = ['DenseASPP', 'NetSpec', 'Scores', 'label_scores']

@@ -17,7 +17,7 @@ HEADER = os.path.join(os.path.dirname(HERE), 'include', 'dsaspp.h')
 LIB_PATH = os.environ.get('DSASPP_LIB_PATH') or os.path.join(HERE, 'libdsaspp.so')
 
 _SCALARS = {
-    'int32_t': ctypes.c_int32, 'int64_t': ctypes.c_int64, 'float': ctypes.c_float,
+    'int32_t': ctypes.c_int32, 'int64_t': ctypes.c_int64, 'float': ctypes.c_float, 'double': ctypes.c_double,
     'uint8_t': ctypes.c_uint8, 'int': ctypes.c_int,
 }
 
@@ -92,6 +92,12 @@ up2_desc = STRUCTS['dsaspp_up2_desc']
 dwbwd_desc = STRUCTS['dsaspp_dwbwd_desc']
 col2im_desc = STRUCTS['dsaspp_col2im_desc']
 stem7_desc = STRUCTS['dsaspp_stem7_desc']
+grad_range = STRUCTS['dsaspp_grad_range']
+clip_desc = STRUCTS['dsaspp_clip_desc']
+adam_clip_desc = STRUCTS['dsaspp_adam_clip_desc']
+scores_desc = STRUCTS['dsaspp_scores_desc']
+scores8_desc = STRUCTS['dsaspp_scores8_desc']
+SCORES_MAX_TOP = DEFINES['DSASPP_SCORES_MAX_TOP']
 
 # op name -> (program op code, descriptor struct, direct entry point)
 OPS = {
@@ -128,6 +134,13 @@ OPS = {
     # direct calls only (not recordable in a program)
     'confusion': (None, conf_desc, 'dsaspp_upsample8_confusion'),
     'preprocess': (None, prep_desc, 'dsaspp_preprocess'),
+    'scores_fwd': (None, scores_desc, 'dsaspp_scores_fwd'),
+    'scores_bwd': (None, scores_desc, 'dsaspp_scores_bwd'),
+    'scores8_fwd': (None, scores8_desc, 'dsaspp_scores8_fwd'),
+    'scores8_bwd': (None, scores8_desc, 'dsaspp_scores8_bwd'),
+    'grad_norm_partials': (None, clip_desc, 'dsaspp_grad_norm_partials'),
+    'grad_norm_finish': (None, clip_desc, 'dsaspp_grad_norm_finish'),
+    'clip_scale': (None, clip_desc, 'dsaspp_clip_scale'),
 }
 
 _lib = None
@@ -170,6 +183,11 @@ def load():
                                            ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p]
     lib.dsaspp_stem7_wgrad_workspace_floats.argtypes = [ctypes.c_int32]
     lib.dsaspp_stem7_wgrad_workspace_floats.restype = ctypes.c_int64
+    lib.dsaspp_grad_norm_workspace.argtypes = [ctypes.POINTER(clip_desc)]
+    lib.dsaspp_grad_norm_workspace.restype = ctypes.c_int64
+    lib.dsaspp_adam_step_clipped.argtypes = [ctypes.POINTER(adam_clip_desc), ctypes.POINTER(clip_desc), ctypes.c_void_p]
+    lib.dsaspp_scores8_workspace.argtypes = [ctypes.POINTER(scores8_desc)]
+    lib.dsaspp_scores8_workspace.restype = ctypes.c_int64
     lib.dsaspp_set_comm_cus.argtypes = [ctypes.c_int32]
     lib.dsaspp_set_comm_cus.restype = ctypes.c_int
     lib.dsaspp_get_comm_cus.restype = ctypes.c_int

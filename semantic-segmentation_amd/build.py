@@ -8,7 +8,9 @@ CSRC = os.path.join(HERE, 'csrc')
 ROOT = os.path.dirname(HERE)
 INCLUDE = os.path.join(ROOT, 'include')
 LIB = os.path.join(HERE, 'libdsaspp.so')
-SOURCES = ['conv_mfma.hip', 'dgrad_group.hip', 'dgrad_wide.hip', 'conv_wide.hip', 'wgrad_wide.hip', 'wgrad3x3_strip.hip', 'conv3x3_halo.hip', 'dgrad3x3_fused.hip', 'conv1x1_stream.hip', 'wgrad_mfma.hip', 'wgrad_group.hip', 'elementwise.hip', 'loss.hip', 'optim.hip', 'mobilenet.hip', 'mobilenet_bwd.hip', 'stem_fused.hip', 'fp32_path.hip', 'eval_ops.hip', 'program.hip']
+SOURCES = ['conv_mfma.hip', 'dgrad_group.hip', 'dgrad_wide.hip', 'conv_wide.hip', 'wgrad_wide.hip', 'wgrad3x3_strip.hip', 'conv3x3_halo.hip', 'dgrad3x3_fused.hip', 'conv1x1_stream.hip', 'wgrad_mfma.hip', 'wgrad_group.hip', 'elementwise.hip', 'loss.hip', 'optim.hip', 'mobilenet.hip', 'mobilenet_bwd.hip', 'stem_fused.hip', 'fp32_path.hip', 'eval_ops.hip', 'gradnorm.hip', 'scores.hip', 'scores8.hip', 'program.hip']
+
+HEADERS = ['common.h', 'elem.h', 'softrow.h']
 
 
 def _hipcc():
@@ -20,6 +22,11 @@ def _hipcc():
 
 # compile flags of the product build: part of the source hash, so that a change here rebuilds the library
 FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-Wall', '-Wno-unused-function']
+# Sources compiled without packed fp32 instructions (v_pk_add/mul/fma_f32): some of their forms have returned wrong values on
+# this hardware, and streaming kernels gain nothing from them.  The sources not listed were tuned and tested with them, down
+# to register budgets and hand-counted waits that another instruction selection would upset.
+NO_PACKED_FP32 = ('gradnorm.hip', 'scores.hip', 'scores8.hip')
+NO_PACKED_FLAGS = ['-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
 
 
 def source_hash(extra_flags=()):
@@ -29,7 +36,8 @@ def source_hash(extra_flags=()):
     import hashlib
     h = hashlib.sha256()
     h.update(' '.join(FLAGS + list(extra_flags)).encode())
-    for path in [os.path.join(CSRC, s) for s in SOURCES] + [os.path.join(CSRC, 'common.h'), os.path.join(INCLUDE, 'dsaspp.h')]:
+    h.update(' '.join([*NO_PACKED_FP32, *NO_PACKED_FLAGS]).encode())
+    for path in [os.path.join(CSRC, s) for s in SOURCES] + [os.path.join(CSRC, n) for n in HEADERS] + [os.path.join(INCLUDE, 'dsaspp.h')]:
         h.update(os.path.basename(path).encode())
         h.update(open(path, 'rb').read())
     return h.hexdigest()[:16]
@@ -64,6 +72,8 @@ def build_library(force=False, verbose=False, extra_flags=(), out=None):
         obj = src[:-4] + ('.o' if out is None else '.%s.o' % sh)
         objs.append(obj)
         cmd = [_hipcc(), *FLAGS, '-I', INCLUDE, '-I', CSRC, *extra_flags, '-c', src, '-o', obj]
+        if os.path.basename(src) in NO_PACKED_FP32:
+            cmd[1:1] = NO_PACKED_FLAGS
         if src.endswith('program.hip'):
             cmd.insert(-4, '-DDSASPP_SOURCE_HASH="%s"' % sh)
         if verbose:

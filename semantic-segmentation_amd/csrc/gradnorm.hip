@@ -1,0 +1,307 @@
+// Global gradient norm over many tensors, clipping by it, and the Adam update with the clip coefficient applied on the fly.
+//
+//   norm = scale * sqrt(sum g^2) (or scale * max |g|),  coef = min(1, max_norm / (norm + 1e-6)),  g <- g * coef
+//
+// Bound by HBM: the norm reads every gradient once, the second pass reads and writes it.  Two launches per call: the first
+// leaves one fp64 partial per block, and every block of the second adds up the same partials in the same order and so knows
+// the coefficient without a third launch, an atomic or a flag.
+#include "elem.h"
+#include <math.h>
+
+namespace {
+
+constexpr int MAX_RANGES = 180;           // ranges that travel in the kernel arguments of one launch (3.6 of 4 KB)
+constexpr int CHUNK = 8192;               // elements of one range that a block takes at a time
+constexpr int MAX_BLOCKS = 2048;          // 8 blocks of 4 waves per CU fill the chip; a block walks several chunks
+constexpr int64_t MAX_ELEMS = (int64_t)CHUNK << 30;
+
+struct Group {
+    void* p[MAX_RANGES];
+    int64_t n[MAX_RANGES];
+    int32_t first[MAX_RANGES + 1];        // first chunk of range i
+    int32_t n_ranges;
+};
+
+__device__ __forceinline__ int find_range(const Group& g, int chunk) {
+    int lo = 0, hi = g.n_ranges - 1;      // last range whose first chunk is <= chunk
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (g.first[mid] <= chunk) lo = mid; else hi = mid - 1;
+    }
+    return lo;
+}
+
+// max that keeps a NaN (fmax drops it)
+__device__ __forceinline__ double max_nan(double a, double b) { return (b > a || b != b) ? b : a; }
+
+template <bool MAXNORM>
+__device__ __forceinline__ double join(double a, double b) { return MAXNORM ? (a != a ? a : max_nan(a, b)) : a + b; }
+
+// The same value in every lane of the block; a fixed order of additions.  `lds`: 4 doubles.
+template <bool MAXNORM>
+__device__ __forceinline__ double block_join(double v, double* lds) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) v = join<MAXNORM>(v, __shfl_xor(v, o, 64));
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return join<MAXNORM>(join<MAXNORM>(lds[0], lds[1]), join<MAXNORM>(lds[2], lds[3]));
+}
+
+template <int DT, bool MAXNORM>
+__global__ __launch_bounds__(256) void partials_kernel(const Group g, double* ws) {
+    typedef Elem<DT> E;
+    __shared__ double lds[4];
+    const int n_chunks = g.first[g.n_ranges];
+    double acc[4] = {0.0, 0.0, 0.0, 0.0};
+    auto take = [&](int k, float x) {
+        if (MAXNORM) acc[k] = join<true>(acc[k], (double)fabsf(x));
+        else acc[k] = __builtin_fma((double)x, (double)x, acc[k]);      // the product is exact: 24 + 24 bits
+    };
+    for (int ch = blockIdx.x; ch < n_chunks; ch += gridDim.x) {
+        const int r = find_range(g, ch);
+        const int64_t off = (int64_t)(ch - g.first[r]) * CHUNK;
+        const int64_t left = g.n[r] - off;
+        const int n = left < CHUNK ? (int)left : CHUNK;
+        const typename E::T* p = reinterpret_cast<const typename E::T*>(g.p[r]) + off;
+        const int nv = n / E::N;
+        for (int i = threadIdx.x; i < nv; i += 256) {
+            const typename E::V v = *reinterpret_cast<const typename E::V*>(p + (int64_t)i * E::N);
+#pragma unroll
+            for (int k = 0; k < E::N; ++k) take(k & 3, E::up(v[k]));
+        }
+        const int t = nv * E::N + (int)threadIdx.x;
+        if (t < n) take(0, E::up(p[t]));                                // fewer than one vector is left
+    }
+    const double v = join<MAXNORM>(join<MAXNORM>(acc[0], acc[1]), join<MAXNORM>(acc[2], acc[3]));
+    const double s = block_join<MAXNORM>(v, lds);
+    if (threadIdx.x == 0) ws[blockIdx.x] = s;
+}
+
+// The norm from the partials of all launches: lane t adds partials t, t + 256, ...; the same in every block.
+template <bool MAXNORM>
+__device__ __forceinline__ double total_norm(const double* ws, int n, float scale, double* lds) {
+    double v = 0.0;
+    for (int i = threadIdx.x; i < n; i += 256) v = join<MAXNORM>(v, ws[i]);
+    v = block_join<MAXNORM>(v, lds);
+    return (double)scale * (MAXNORM ? v : sqrt(v));
+}
+
+__device__ __forceinline__ float clip_coef(double norm, float max_norm) {
+    // an infinite threshold never clips (inf / inf would be NaN); a NaN norm stays NaN
+    if (norm == norm && max_norm == INFINITY) return 1.f;
+    const double c = (double)max_norm / (norm + 1e-6);
+    return c > 1.0 ? 1.f : (float)c;
+}
+
+__device__ __forceinline__ double any_norm(const double* ws, int n, int norm_type, float scale, double* lds) {
+    return norm_type == 2 ? total_norm<false>(ws, n, scale, lds) : total_norm<true>(ws, n, scale, lds);
+}
+
+__global__ __launch_bounds__(256) void finish_kernel(const double* ws, int n, int norm_type, float scale, float* norm) {
+    __shared__ double lds[4];
+    const double v = any_norm(ws, n, norm_type, scale, lds);
+    if (threadIdx.x == 0) norm[0] = (float)v;
+}
+
+template <int DT>
+__global__ __launch_bounds__(256) void scale_kernel(const Group g, const double* ws, int n_ws, int norm_type, float max_norm, float* norm) {
+    typedef Elem<DT> E;
+    __shared__ double lds[4];
+    const double total = any_norm(ws, n_ws, norm_type, 1.f, lds);
+    if (blockIdx.x == 0 && threadIdx.x == 0) norm[0] = (float)total;
+    const float coef = clip_coef(total, max_norm);
+    if (coef == 1.f) return;              // x * 1 is x
+    const int n_chunks = g.first[g.n_ranges];
+    for (int ch = blockIdx.x; ch < n_chunks; ch += gridDim.x) {
+        const int r = find_range(g, ch);
+        const int64_t off = (int64_t)(ch - g.first[r]) * CHUNK;
+        const int64_t left = g.n[r] - off;
+        const int n = left < CHUNK ? (int)left : CHUNK;
+        typename E::T* p = reinterpret_cast<typename E::T*>(g.p[r]) + off;
+        const int nv = n / E::N;
+        for (int i = threadIdx.x; i < nv; i += 256) {
+            typename E::V* q = reinterpret_cast<typename E::V*>(p + (int64_t)i * E::N);
+            typename E::V v = *q;
+#pragma unroll
+            for (int k = 0; k < E::N; ++k) v[k] = E::down(E::up(v[k]) * coef);
+            *q = v;
+        }
+        const int t = nv * E::N + (int)threadIdx.x;
+        if (t < n) p[t] = E::down(E::up(p[t]) * coef);
+    }
+}
+
+struct AdamArgs {
+    int64_t n;
+    float* p; const float* g; float* m; float* v;
+    u16* w16;
+    float lr1, beta1, beta1c, beta2, beta2c, bc2s, eps, weight_decay;      // lr / bias correction 1, 1 - beta, sqrt(bias correction 2)
+};
+
+// Adam with coupled L2, as torch.optim.Adam(weight_decay=...), on g * scale * coef.
+__global__ __launch_bounds__(256) void adam_clipped_kernel(const AdamArgs d, const double* ws, int n_ws, int norm_type, float scale, float max_norm,
+                                                           float* norm) {
+    __shared__ double lds[4];
+    const double total = any_norm(ws, n_ws, norm_type, scale, lds);
+    if (blockIdx.x == 0 && threadIdx.x == 0) norm[0] = (float)total;
+    const float gs = scale * clip_coef(total, max_norm);
+    auto update = [&](float& p, const float gr, float& m, float& v) {
+        const float g = gr * gs + d.weight_decay * p;
+        m = d.beta1 * m + d.beta1c * g;
+        v = d.beta2 * v + d.beta2c * g * g;
+        p -= d.lr1 * (m / (sqrtf(v) / d.bc2s + d.eps));
+    };
+    u16* w16 = d.w16;
+    const int64_t nv = d.n / 4;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < nv; i += (int64_t)gridDim.x * 256) {
+        f32x4u* qp = reinterpret_cast<f32x4u*>(d.p) + i;
+        f32x4u* qm = reinterpret_cast<f32x4u*>(d.m) + i;
+        f32x4u* qv = reinterpret_cast<f32x4u*>(d.v) + i;
+        f32x4u p = *qp, m = *qm, v = *qv;
+        const f32x4u g = *(reinterpret_cast<const f32x4u*>(d.g) + i);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            float pk = p[k], mk = m[k], vk = v[k];
+            update(pk, g[k], mk, vk);
+            p[k] = pk; m[k] = mk; v[k] = vk;
+        }
+        *qp = p; *qm = m; *qv = v;
+        if (w16) {
+            typedef uint32_t u32x2u __attribute__((ext_vector_type(2), aligned(2)));
+            u32x2u o;
+            o[0] = pack_bf2(p[0], p[1]);
+            o[1] = pack_bf2(p[2], p[3]);
+            *reinterpret_cast<u32x2u*>(w16 + i * 4) = o;
+        }
+    }
+    const int64_t t = nv * 4 + threadIdx.x;
+    if (blockIdx.x == 0 && t < d.n) {
+        update(d.p[t], d.g[t], d.m[t], d.v[t]);
+        if (w16) w16[t] = (u16)f2bf_bits(d.p[t]);
+    }
+}
+
+int blocks_for(int64_t chunks) { return (int)(chunks < MAX_BLOCKS ? chunks : MAX_BLOCKS); }
+
+// Calls fn(dtype, group) for every launch the ranges need: up to MAX_RANGES ranges of one type each.
+template <typename F>
+void for_each_group(const dsaspp_clip_desc& d, F fn) {
+    for (int dt = 0; dt < 3; ++dt) {
+        Group g;
+        g.n_ranges = 0;
+        g.first[0] = 0;
+        for (int i = 0; i < d.n_ranges; ++i) {
+            const dsaspp_grad_range& r = d.ranges[i];
+            if (r.dtype != dt) continue;
+            const int64_t chunks = (r.n + CHUNK - 1) / CHUNK;
+            if (g.n_ranges == MAX_RANGES || (g.n_ranges > 0 && g.first[g.n_ranges] + chunks > (1ll << 30))) {
+                fn(dt, g);
+                g.n_ranges = 0;
+            }
+            g.p[g.n_ranges] = r.p;
+            g.n[g.n_ranges] = r.n;
+            g.first[g.n_ranges + 1] = g.first[g.n_ranges] + (int32_t)chunks;
+            ++g.n_ranges;
+        }
+        if (g.n_ranges) fn(dt, g);
+    }
+}
+
+int check(const dsaspp_clip_desc* d, const char* who) {
+    DS_REQUIRE(d, "%s: null descriptor", who);
+    DS_REQUIRE(d->n_ranges >= 0 && (d->n_ranges == 0 || d->ranges), "%s: bad list of ranges", who);
+    DS_REQUIRE(d->norm_type == 2 || d->norm_type == 0, "%s: norm_type must be 2 (Euclidean) or 0 (largest magnitude), got %d", who, d->norm_type);
+    DS_REQUIRE(d->scale > 0.f && d->scale < INFINITY, "%s: scale must be positive and finite", who);
+    for (int i = 0; i < d->n_ranges; ++i) {
+        const dsaspp_grad_range& r = d->ranges[i];
+        DS_REQUIRE(r.dtype >= 0 && r.dtype <= 2, "%s: range %d has dtype %d (0 = bf16, 1 = fp32, 2 = fp16)", who, i, r.dtype);
+        DS_REQUIRE(r.p && r.n > 0 && r.n <= MAX_ELEMS, "%s: range %d is empty, too long or null", who, i);
+        DS_REQUIRE(((uintptr_t)r.p & (r.dtype == 1 ? 3 : 1)) == 0, "%s: range %d is not aligned to its element type", who, i);
+    }
+    return 0;
+}
+
+int64_t n_partials(const dsaspp_clip_desc& d) {
+    int64_t n = 0;
+    for_each_group(d, [&](int, const Group& g) { n += blocks_for(g.first[g.n_ranges]); });
+    return n;
+}
+
+int check_ws(const dsaspp_clip_desc* d, const char* who, int64_t* used) {
+    if (int rc = check(d, who)) return rc;
+    *used = n_partials(*d);
+    DS_REQUIRE(*used < (1ll << 31), "%s: too many ranges", who);
+    DS_REQUIRE(*used == 0 || (d->ws && d->ws_len >= *used && ((uintptr_t)d->ws & 7) == 0), "%s: the workspace needs %lld doubles", who, (long long)*used);
+    return 0;
+}
+
+}  // namespace
+
+extern "C" int64_t dsaspp_grad_norm_workspace(const dsaspp_clip_desc* d) {
+    if (check(d, "grad_norm_workspace")) return -1;
+    return n_partials(*d);
+}
+
+extern "C" int dsaspp_grad_norm_partials(const dsaspp_clip_desc* d, dsaspp_stream_t stream) {
+    int64_t used = 0;
+    if (int rc = check_ws(d, "grad_norm_partials", &used)) return rc;
+    double* ws = d->ws;
+    hipStream_t s = (hipStream_t)stream;
+    for_each_group(*d, [&](int dt, const Group& g) {
+        const int nb = blocks_for(g.first[g.n_ranges]);
+#define PARTIALS(DT)                                                                                                       \
+        if (d->norm_type == 2) hipLaunchKernelGGL((partials_kernel<DT, false>), dim3(nb), dim3(256), 0, s, g, ws);         \
+        else hipLaunchKernelGGL((partials_kernel<DT, true>), dim3(nb), dim3(256), 0, s, g, ws)
+        if (dt == 0) { PARTIALS(0); } else if (dt == 1) { PARTIALS(1); } else { PARTIALS(2); }
+#undef PARTIALS
+        ws += nb;
+    });
+    DS_LAUNCH_CHECK("grad_norm_partials");
+    return 0;
+}
+
+extern "C" int dsaspp_grad_norm_finish(const dsaspp_clip_desc* d, dsaspp_stream_t stream) {
+    int64_t used = 0;
+    if (int rc = check_ws(d, "grad_norm_finish", &used)) return rc;
+    DS_REQUIRE(d->norm, "grad_norm_finish: null output");
+    hipLaunchKernelGGL(finish_kernel, dim3(1), dim3(256), 0, (hipStream_t)stream, d->ws, (int)used, d->norm_type, d->scale, d->norm);
+    DS_LAUNCH_CHECK("grad_norm_finish");
+    return 0;
+}
+
+extern "C" int dsaspp_clip_scale(const dsaspp_clip_desc* d, dsaspp_stream_t stream) {
+    int64_t used = 0;
+    if (int rc = check_ws(d, "clip_scale", &used)) return rc;
+    DS_REQUIRE(d->norm, "clip_scale: null output");
+    DS_REQUIRE(d->scale == 1.f, "clip_scale: scale must be 1");
+    DS_REQUIRE(d->max_norm >= 0.f, "clip_scale: max_norm must be >= 0");
+    if (d->n_ranges == 0) return dsaspp_grad_norm_finish(d, stream);
+    hipStream_t s = (hipStream_t)stream;
+    for_each_group(*d, [&](int dt, const Group& g) {
+        const int nb = blocks_for(g.first[g.n_ranges]);
+        if (dt == 0) hipLaunchKernelGGL(scale_kernel<0>, dim3(nb), dim3(256), 0, s, g, d->ws, (int)used, d->norm_type, d->max_norm, d->norm);
+        else if (dt == 1) hipLaunchKernelGGL(scale_kernel<1>, dim3(nb), dim3(256), 0, s, g, d->ws, (int)used, d->norm_type, d->max_norm, d->norm);
+        else hipLaunchKernelGGL(scale_kernel<2>, dim3(nb), dim3(256), 0, s, g, d->ws, (int)used, d->norm_type, d->max_norm, d->norm);
+    });
+    DS_LAUNCH_CHECK("clip_scale");
+    return 0;
+}
+
+extern "C" int dsaspp_adam_step_clipped(const dsaspp_adam_clip_desc* a, const dsaspp_clip_desc* c, dsaspp_stream_t stream) {
+    int64_t used = 0;
+    DS_REQUIRE(a && a->n > 0 && a->n <= MAX_ELEMS, "adam_step_clipped: n must be positive");
+    DS_REQUIRE(a->p && a->g && a->m && a->v && a->step >= 1, "adam_step_clipped: bad descriptor");
+    DS_REQUIRE((((uintptr_t)a->p | (uintptr_t)a->g | (uintptr_t)a->m | (uintptr_t)a->v) & 3) == 0 && ((uintptr_t)a->w16 & 1) == 0,
+               "adam_step_clipped: buffers must be aligned to their element type");
+    if (int rc = check_ws(c, "adam_step_clipped", &used)) return rc;
+    DS_REQUIRE(c->norm && c->max_norm >= 0.f, "adam_step_clipped: null output or negative max_norm");
+    const AdamArgs d = {a->n, a->p, a->g, a->m, a->v, reinterpret_cast<u16*>(a->w16),
+                        (float)(a->lr / (1.0 - pow(a->beta1, (double)a->step))), (float)a->beta1, (float)(1.0 - a->beta1), (float)a->beta2,
+                        (float)(1.0 - a->beta2), (float)sqrt(1.0 - pow(a->beta2, (double)a->step)), (float)a->eps, (float)a->weight_decay};
+    int64_t nb = (a->n / 4 + 255) / 256;
+    nb = nb < 1 ? 1 : nb > MAX_BLOCKS ? MAX_BLOCKS : nb;
+    hipLaunchKernelGGL(adam_clipped_kernel, dim3((unsigned)nb), dim3(256), 0, (hipStream_t)stream, d, c->ws, (int)used, c->norm_type, c->scale,
+                       c->max_norm, c->norm);
+    DS_LAUNCH_CHECK("adam_step_clipped");
+    return 0;
+}

@@ -1,0 +1,422 @@
+// Log probability of a given label, entropy and the most probable classes of every row of a tensor of logits, and the gradient.
+//
+//   log_p[c] = z[c] - m - log s,  H = log s - (sum (z-m) e^(z-m)) / s,  m = max z, s = sum e^(z-m)
+//   dz[c] = a [c == label] + sum_j t_j [c == top_j] - p[c] A - b p[c] (log_p[c] + H),   A = a + sum t_j
+//
+// Both directions are one pass over the logits and bound by HBM: maximum, sums and the K largest run along with the pass; the
+// backward pass gets m, log s and H from the forward pass and never sums.  Two layouts, two kernels each: "rows" (the classes are
+// contiguous: a group of lanes shares a row and reads 16 bytes per lane) and "planes" (class stride other than 1, NCHW: a lane owns
+// P neighbouring pixels and walks the classes).
+#include "softrow.h"
+
+namespace {
+
+struct Args {
+    dsaspp_scores_desc d;
+    int64_t rows, plane;                  // d0*d1*d2, d1*d2
+};
+
+struct Row {
+    int64_t i0, rem;                      // index along d0, index inside [d1][d2]
+    int64_t off;                          // of class 0, in elements
+};
+
+__device__ __forceinline__ Row row_of(const Args& a, int64_t row) {
+    Row r;
+    if (a.plane == 1) {
+        r.i0 = row;
+        r.rem = 0;
+        r.off = row * a.d.s0;
+    } else {
+        r.i0 = row / a.plane;
+        r.rem = row - r.i0 * a.plane;
+        const int64_t i1 = r.rem / a.d.d2;
+        r.off = r.i0 * a.d.s0 + i1 * a.d.s1 + (r.rem - i1 * a.d.d2) * a.d.s2;
+    }
+    return r;
+}
+
+// class of the row's label, -1 for a row without one
+__device__ __forceinline__ int label_of(const dsaspp_scores_desc& d, int64_t row) {
+    if (!d.labels) return -1;
+    const int64_t l = d.labels[row];
+    return l != d.ignore_index && l >= 0 && l < d.n_class ? (int)l : -1;
+}
+
+__device__ __forceinline__ float label_log_p(int label, float z, const Soft& s, float log_s) {
+    return label < 0 ? 0.f : s.empty() ? -INFINITY : (z - s.m) - log_s;
+}
+
+// m and log s for the backward pass; a row with nothing but -inf gets log s = +inf, which makes every p 0
+__device__ __forceinline__ void store_stats(float* stats, int64_t row, const Soft& s, float log_s) {
+    stats[2 * row] = s.empty() ? 0.f : s.m;
+    stats[2 * row + 1] = s.empty() ? INFINITY : log_s;
+}
+
+// ---------------------------------------------------------------- rows: TPR lanes share a row
+template <int DT, int K, int TPR>
+__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rows_fwd_kernel(const Args a) {
+    typedef Elem<DT> E;
+    constexpr int BLOCK = TPR > 256 ? TPR : 256, RPB = BLOCK / TPR, WAVES = TPR > 64 ? TPR / 64 : 1;
+    __shared__ float ls[WAVES][3];
+    __shared__ float lv[WAVES][K > 0 ? K : 1];
+    __shared__ int li[WAVES][K > 0 ? K : 1];
+    const dsaspp_scores_desc& d = a.d;
+    const int V = d.n_class, lane = threadIdx.x % TPR;
+    for (int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR; row < a.rows; row += (int64_t)gridDim.x * RPB) {
+        const Row r = row_of(a, row);
+        const typename E::T* z = reinterpret_cast<const typename E::T*>(d.logits) + r.off;
+        const int label = label_of(d, row);
+        const float zl = label >= 0 ? E::up(z[label]) : 0.f;
+        Soft s;
+        Top<K> top;
+        s.clear();
+        top.clear();
+        auto take = [&](const float* f, int n, int c) {
+            float mx = f[0];
+#pragma unroll
+            for (int k = 1; k < n; ++k) mx = fmaxf(mx, f[k]);
+            if (mx > s.m) s.shift_to(mx);
+#pragma unroll
+            for (int k = 0; k < n; ++k) {
+                s.add(f[k]);
+                top.offer(f[k], c + k);
+            }
+        };
+        const int full = V / E::N * E::N;
+        for (int c = lane * E::N; c < full; c += TPR * E::N) {
+            const typename E::V v = *reinterpret_cast<const typename E::V*>(z + c);
+            float f[E::N];
+#pragma unroll
+            for (int k = 0; k < E::N; ++k) f[k] = E::up(v[k]);
+            take(f, E::N, c);
+        }
+        if (full + lane < V) {            // fewer than E::N <= 8 <= TPR are left
+            const float f = E::up(z[full + lane]);
+            take(&f, 1, full + lane);
+        }
+        constexpr int G = TPR < 64 ? TPR : 64;
+#pragma unroll
+        for (int o = 1; o < G; o <<= 1) s.join(__shfl_xor(s.m, o, 64), __shfl_xor(s.s, o, 64), __shfl_xor(s.t, o, 64));
+        top.template join_lanes<G>();
+        if (TPR > 64) {
+            const int wave = threadIdx.x >> 6, wl = threadIdx.x & 63;
+            __syncthreads();              // the lists of the block's previous row have been read
+            if (wl == 0) {
+                ls[wave][0] = s.m; ls[wave][1] = s.s; ls[wave][2] = s.t;
+#pragma unroll
+                for (int j = 0; j < K; ++j) { lv[wave][j] = top.v[j]; li[wave][j] = top.i[j]; }
+            }
+            __syncthreads();
+            if (wave != 0) continue;      // to the next row's first barrier, as wave 0 does after writing
+            s.clear();
+            top.clear();
+            if (wl < WAVES) {
+                s = Soft{ls[wl][0], ls[wl][1], ls[wl][2]};
+#pragma unroll
+                for (int j = 0; j < K; ++j) { top.v[j] = lv[wl][j]; top.i[j] = li[wl][j]; }
+            }
+#pragma unroll
+            for (int o = 1; o < WAVES; o <<= 1) s.join(__shfl_xor(s.m, o, 64), __shfl_xor(s.s, o, 64), __shfl_xor(s.t, o, 64));
+            top.template join_lanes<WAVES>();
+        }
+        const float log_s = logf(s.s);
+        if (lane == 0) {
+            if (d.logp) d.logp[row] = label_log_p(label, zl, s, log_s);
+            if (d.entropy) d.entropy[row] = s.entropy(log_s);
+            if (d.stats) store_stats(d.stats, row, s, log_s);
+#pragma unroll
+            for (int j = 0; j < K; ++j)
+                if (j < d.top_k) {
+                    const int64_t o = (r.i0 * d.top_k + j) * a.plane + r.rem;
+                    d.top_logp[o] = top_log_p(top.v[j], top.i[j], s, log_s);
+                    d.top_class[o] = top_index(top.i[j], s);
+                }
+        }
+    }
+}
+
+// what the gradient of one row needs besides its logits
+template <int K>
+struct Up {
+    float m, log_s, h, a, b, A;
+    float t[K > 0 ? K : 1];
+    int label, top[K > 0 ? K : 1];
+    bool live;
+    __device__ __forceinline__ void load(const dsaspp_scores_desc& d, int64_t plane, int64_t row, int64_t i0, int64_t rem) {
+        m = d.stats[2 * row];
+        log_s = d.stats[2 * row + 1];
+        label = label_of(d, row);
+        a = d.g_logp && label >= 0 ? d.g_logp[d.g_logp_one ? 0 : row] : 0.f;
+        b = d.g_entropy ? d.g_entropy[d.g_entropy_one ? 0 : row] : 0.f;
+        h = d.g_entropy ? d.entropy[row] : 0.f;
+        A = a;
+        live = a != 0.f || b != 0.f;
+#pragma unroll
+        for (int j = 0; j < K; ++j) {
+            t[j] = 0.f;
+            top[j] = -1;
+            if (d.g_top && j < d.top_k) {
+                const int64_t o = (i0 * d.top_k + j) * plane + rem;
+                top[j] = (int)d.top_class[o];
+                const float g = d.g_top[d.g_top_one ? 0 : o];
+                // without alternatives because of a NaN: the gradient is NaN unless nothing flows back
+                t[j] = top[j] >= 0 ? g : (log_s != log_s && g != 0.f) ? log_s : 0.f;
+                A += t[j];
+                live = live || t[j] != 0.f;
+            }
+        }
+        live = live && log_s != INFINITY;      // every class masked out
+    }
+    __device__ __forceinline__ float grad(float z, int c) const {
+        const float lp = (z - m) - log_s, p = __builtin_amdgcn_exp2f(lp * SR_LOG2E);
+        float g = -p * fmaf(b, fmaxf(lp, SR_FAR) + h, A);
+        if (c == label) g += a;
+#pragma unroll
+        for (int j = 0; j < K; ++j)
+            if (c == top[j]) g += t[j];
+        return live ? g : 0.f;
+    }
+};
+
+template <int DT, int K, int TPR>
+__global__ __launch_bounds__(256) void rows_bwd_kernel(const Args a) {
+    typedef Elem<DT> E;
+    constexpr int RPB = 256 / TPR;
+    const dsaspp_scores_desc& d = a.d;
+    const int V = d.n_class, lane = threadIdx.x % TPR;
+    for (int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR; row < a.rows; row += (int64_t)gridDim.x * RPB) {
+        const Row r = row_of(a, row);
+        const typename E::T* z = reinterpret_cast<const typename E::T*>(d.logits) + r.off;
+        typename E::T* o = reinterpret_cast<typename E::T*>(d.dlogits) + row * V;
+        Up<K> u;
+        u.load(d, a.plane, row, r.i0, r.rem);
+        const int full = V / E::N * E::N;
+        for (int c = lane * E::N; c < full; c += TPR * E::N) {
+            const typename E::V v = *reinterpret_cast<const typename E::V*>(z + c);
+            typename E::V w;
+#pragma unroll
+            for (int k = 0; k < E::N; ++k) w[k] = E::down(u.grad(E::up(v[k]), c + k));
+            *reinterpret_cast<typename E::V*>(o + c) = w;
+        }
+        if (full + lane < V) o[full + lane] = E::down(u.grad(E::up(z[full + lane]), full + lane));
+    }
+}
+
+// ---------------------------------------------------------------- planes: a lane owns P neighbouring pixels
+// P pixels of one class; np < P only at the end of a row of pixels (lanes past the end hold -inf)
+template <int DT, int P>
+__device__ __forceinline__ void load_px(const typename Elem<DT>::T* p, int np, float (&f)[P]) {
+    typedef Elem<DT> E;
+    if (P == 1) {
+        f[0] = E::up(p[0]);
+    } else if (np == P) {
+        const typename E::V4 v = *reinterpret_cast<const typename E::V4*>(p);
+#pragma unroll
+        for (int k = 0; k < P; ++k) f[k] = E::up(v[k & 3]);
+    } else {
+#pragma unroll
+        for (int k = 0; k < P; ++k) f[k] = k < np ? E::up(p[k]) : -INFINITY;
+    }
+}
+
+constexpr int PU = 4;                     // classes a lane has in flight
+
+template <int DT, int K, int P>
+__global__ __launch_bounds__(256) void planes_fwd_kernel(const Args a, const int64_t groups, const int64_t per_row) {
+    typedef Elem<DT> E;
+    const dsaspp_scores_desc& d = a.d;
+    const int V = d.n_class;
+    for (int64_t g = (int64_t)blockIdx.x * 256 + threadIdx.x; g < groups; g += (int64_t)gridDim.x * 256) {
+        const int64_t line = g / per_row, i2 = (g - line * per_row) * P;
+        const int64_t row = line * d.d2 + i2;
+        const int np = d.d2 - i2 < P ? (int)(d.d2 - i2) : P;
+        const Row r = row_of(a, row);
+        const typename E::T* z = reinterpret_cast<const typename E::T*>(d.logits) + r.off;
+        Soft s[P];
+        Top<K> top[P];
+#pragma unroll
+        for (int q = 0; q < P; ++q) { s[q].clear(); top[q].clear(); }
+        int c = 0;
+        for (; c + PU <= V; c += PU) {
+            float f[PU][P];
+#pragma unroll
+            for (int u = 0; u < PU; ++u) load_px<DT, P>(z + (c + u) * d.sc, np, f[u]);
+#pragma unroll
+            for (int q = 0; q < P; ++q) {
+                float mx = f[0][q];
+#pragma unroll
+                for (int u = 1; u < PU; ++u) mx = fmaxf(mx, f[u][q]);
+                if (mx > s[q].m) s[q].shift_to(mx);
+#pragma unroll
+                for (int u = 0; u < PU; ++u) {
+                    s[q].add(f[u][q]);
+                    top[q].offer(f[u][q], c + u);
+                }
+            }
+        }
+        for (; c < V; ++c) {
+            float f[P];
+            load_px<DT, P>(z + c * d.sc, np, f);
+#pragma unroll
+            for (int q = 0; q < P; ++q) {
+                if (f[q] > s[q].m) s[q].shift_to(f[q]);
+                s[q].add(f[q]);
+                top[q].offer(f[q], c);
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < P; ++q) {
+            if (q >= np) break;
+            const float log_s = logf(s[q].s);
+            if (d.logp) {
+                const int label = label_of(d, row + q);
+                const float zl = label >= 0 ? E::up(z[label * d.sc + q]) : 0.f;
+                d.logp[row + q] = label_log_p(label, zl, s[q], log_s);
+            }
+            if (d.entropy) d.entropy[row + q] = s[q].entropy(log_s);
+            if (d.stats) store_stats(d.stats, row + q, s[q], log_s);
+#pragma unroll
+            for (int j = 0; j < K; ++j)
+                if (j < d.top_k) {
+                    const int64_t o = (r.i0 * d.top_k + j) * a.plane + r.rem + q;
+                    d.top_logp[o] = top_log_p(top[q].v[j], top[q].i[j], s[q], log_s);
+                    d.top_class[o] = top_index(top[q].i[j], s[q]);
+                }
+        }
+    }
+}
+
+template <int DT, int K, int P>
+__global__ __launch_bounds__(256) void planes_bwd_kernel(const Args a, const int64_t groups, const int64_t per_row) {
+    typedef Elem<DT> E;
+    const dsaspp_scores_desc& d = a.d;
+    const int V = d.n_class;
+    for (int64_t g = (int64_t)blockIdx.x * 256 + threadIdx.x; g < groups; g += (int64_t)gridDim.x * 256) {
+        const int64_t line = g / per_row, i2 = (g - line * per_row) * P;
+        const int64_t row = line * d.d2 + i2;
+        const int np = d.d2 - i2 < P ? (int)(d.d2 - i2) : P;
+        const Row r = row_of(a, row);
+        const typename E::T* z = reinterpret_cast<const typename E::T*>(d.logits) + r.off;
+        typename E::T* o = reinterpret_cast<typename E::T*>(d.dlogits) + r.i0 * V * a.plane + r.rem;
+        Up<K> u[P];
+#pragma unroll
+        for (int q = 0; q < P; ++q) u[q].load(d, a.plane, q < np ? row + q : row, r.i0, q < np ? r.rem + q : r.rem);
+#pragma unroll PU
+        for (int c = 0; c < V; ++c) {
+            float f[P];
+            load_px<DT, P>(z + c * d.sc, np, f);
+#pragma unroll
+            for (int q = 0; q < P; ++q) f[q] = u[q].grad(f[q], c);
+            typename E::T* oc = o + c * a.plane;
+            if (P > 1 && np == P) {
+                typename E::V4 w;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) w[q] = E::down(f[q < P ? q : 0]);
+                *reinterpret_cast<typename E::V4*>(oc) = w;
+            } else {
+#pragma unroll
+                for (int q = 0; q < P; ++q)
+                    if (q < np) oc[q] = E::down(f[q]);
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------- host side
+int check(const dsaspp_scores_desc* d, const char* who, Args* a) {
+    DS_REQUIRE(d, "%s: null descriptor", who);
+    DS_REQUIRE(d->dtype >= 0 && d->dtype <= 2, "%s: dtype must be 0 (bf16), 1 (fp32) or 2 (fp16), got %d", who, d->dtype);
+    DS_REQUIRE(d->n_class > 0 && d->n_class < (1 << 30), "%s: n_class must be in [1, 2^30)", who);
+    DS_REQUIRE(d->top_k >= 0 && d->top_k <= DSASPP_SCORES_MAX_TOP && d->top_k <= d->n_class, "%s: top_k must be in [0, %d] and at most n_class, got %d", who,
+               DSASPP_SCORES_MAX_TOP, d->top_k);
+    DS_REQUIRE(d->d0 > 0 && d->d1 > 0 && d->d2 > 0 && d->d0 < (1ll << 40) / d->d1 && d->d0 * d->d1 < (1ll << 40) / d->d2, "%s: bad row counts", who);
+    DS_REQUIRE(d->s0 >= 0 && d->s1 >= 0 && d->s2 >= 0 && d->sc >= 0, "%s: negative stride", who);
+    DS_REQUIRE(d->logits, "%s: null logits", who);
+    DS_REQUIRE(((uintptr_t)d->logits & (d->dtype == 1 ? 3 : 1)) == 0, "%s: logits are not aligned to their element type", who);
+    a->d = *d;
+    a->plane = d->d1 * d->d2;
+    a->rows = d->d0 * a->plane;
+    return 0;
+}
+
+unsigned grid_for(int64_t blocks) { return (unsigned)(blocks < (1 << 20) ? blocks : (1 << 20)); }
+
+// Pixels per lane: 4 where they are contiguous and there are enough of them to fill the chip (256 CUs of 8 waves) all the same.
+int px_per_lane(const Args& a) { return a.d.s2 == 1 && a.d.d2 >= 4 && a.rows >= 4 * 256 * 512 ? 4 : 1; }
+
+template <int DT, int K, bool BWD>
+void launch_planes(const Args& a, hipStream_t s) {
+    const int P = px_per_lane(a);
+    const int64_t per_row = (a.d.d2 + P - 1) / P, groups = a.d.d0 * a.d.d1 * per_row;
+    const dim3 grid(grid_for((groups + 255) / 256)), block(256);
+    if (BWD) {
+        if (P == 4) hipLaunchKernelGGL((planes_bwd_kernel<DT, K, 4>), grid, block, 0, s, a, groups, per_row);
+        else hipLaunchKernelGGL((planes_bwd_kernel<DT, K, 1>), grid, block, 0, s, a, groups, per_row);
+    } else {
+        if (P == 4) hipLaunchKernelGGL((planes_fwd_kernel<DT, K, 4>), grid, block, 0, s, a, groups, per_row);
+        else hipLaunchKernelGGL((planes_fwd_kernel<DT, K, 1>), grid, block, 0, s, a, groups, per_row);
+    }
+}
+
+template <int DT, int K, int TPR, bool BWD>
+void launch_rows_tpr(const Args& a, hipStream_t s) {
+    constexpr int T = BWD && TPR > 256 ? 256 : TPR, BLOCK = T > 256 ? T : 256, RPB = BLOCK / T;
+    const dim3 grid(grid_for((a.rows + RPB - 1) / RPB)), block(BLOCK);
+    if (BWD) hipLaunchKernelGGL((rows_bwd_kernel<DT, K, T>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((rows_fwd_kernel<DT, K, TPR>), grid, block, 0, s, a);
+}
+
+template <int DT, int K, bool BWD>
+void launch_rows(const Args& a, hipStream_t s) {
+    const int V = a.d.n_class;
+    if (V <= 64) launch_rows_tpr<DT, K, 8, BWD>(a, s);
+    else if (V <= 1024) launch_rows_tpr<DT, K, 64, BWD>(a, s);
+    else if (V <= 8192 || a.rows >= 1024) launch_rows_tpr<DT, K, 256, BWD>(a, s);
+    else launch_rows_tpr<DT, K, 1024, BWD>(a, s);
+}
+
+template <int DT, bool BWD>
+void launch_k(const Args& a, int k, hipStream_t s) {
+    const bool rows = a.d.sc == 1 || a.d.n_class == 1;
+#define LAUNCH(K) rows ? launch_rows<DT, K, BWD>(a, s) : launch_planes<DT, K, BWD>(a, s)
+    if (k == 0) LAUNCH(0);
+    else if (k == 1) LAUNCH(1);
+    else if (k <= 3) LAUNCH(3);
+    else LAUNCH(8);
+#undef LAUNCH
+}
+
+}  // namespace
+
+extern "C" int dsaspp_scores_fwd(const dsaspp_scores_desc* d, dsaspp_stream_t stream) {
+    Args a;
+    if (int rc = check(d, "scores_fwd", &a)) return rc;
+    DS_REQUIRE(!d->logp || d->labels, "scores_fwd: logp needs labels");
+    DS_REQUIRE((d->top_k > 0) == (d->top_logp != nullptr) && (d->top_k > 0) == (d->top_class != nullptr), "scores_fwd: top_logp and top_class go with top_k > 0");
+    DS_REQUIRE(d->logp || d->entropy || d->stats || d->top_k, "scores_fwd: nothing to compute");
+    hipStream_t s = (hipStream_t)stream;
+    if (d->dtype == 0) launch_k<0, false>(a, d->top_k, s);
+    else if (d->dtype == 1) launch_k<1, false>(a, d->top_k, s);
+    else launch_k<2, false>(a, d->top_k, s);
+    DS_LAUNCH_CHECK("scores_fwd");
+    return 0;
+}
+
+extern "C" int dsaspp_scores_bwd(const dsaspp_scores_desc* d, dsaspp_stream_t stream) {
+    Args a;
+    if (int rc = check(d, "scores_bwd", &a)) return rc;
+    DS_REQUIRE(d->stats && d->dlogits, "scores_bwd: null stats or gradient");
+    DS_REQUIRE(((uintptr_t)d->dlogits & (d->dtype == 1 ? 3 : 1)) == 0, "scores_bwd: dlogits is not aligned to its element type");
+    DS_REQUIRE(d->g_logp || d->g_entropy || d->g_top, "scores_bwd: no upstream gradient");
+    DS_REQUIRE(!d->g_logp || d->labels, "scores_bwd: g_logp needs labels");
+    DS_REQUIRE(!d->g_entropy || d->entropy, "scores_bwd: g_entropy needs the entropy of the forward pass");
+    DS_REQUIRE(!d->g_top || (d->top_k > 0 && d->top_class), "scores_bwd: g_top needs top_class of the forward pass");
+    hipStream_t s = (hipStream_t)stream;
+    const int k = d->g_top ? d->top_k : 0;
+    if (d->dtype == 0) launch_k<0, true>(a, k, s);
+    else if (d->dtype == 1) launch_k<1, true>(a, k, s);
+    else launch_k<2, true>(a, k, s);
+    DS_LAUNCH_CHECK("scores_bwd");
+    return 0;
+}

@@ -1,0 +1,98 @@
+// One pass over the logits of a row: running maximum, sum of exponentials, sum for the entropy, and the K largest logits.
+#pragma once
+#include "elem.h"
+#include <float.h>
+
+constexpr float SR_LOG2E = 1.4426950408889634f, SR_LN2 = 0.6931471805599453f;
+constexpr float SR_FAR = -1000.f;         // stands for any difference whose exponential is 0 (below -150) where the two are multiplied
+
+// With d = (z - m) log2 e:  s = sum 2^d,  t = sum d 2^d.  The running maximum starts at the lowest finite value, so a row of
+// nothing but -inf keeps s == 0 and any finite logit makes s >= 1.  A NaN or +inf makes s NaN and nothing takes that back.
+struct Soft {
+    float m, s, t;
+    __device__ __forceinline__ void clear() { m = -FLT_MAX; s = 0.f; t = 0.f; }
+    // change of reference: d -> d + D, so s -> s 2^D and t -> (t + D s) 2^D
+    __device__ __forceinline__ void shift_to(float mn) {
+        const float D = fmaxf((m - mn) * SR_LOG2E, SR_FAR), f = __builtin_amdgcn_exp2f(D);
+        t = fmaf(D, s, t) * f;
+        s *= f;
+        m = mn;
+    }
+    __device__ __forceinline__ void add(float z) {       // z <= m, or -inf, or NaN
+        const float d = (z - m) * SR_LOG2E, e = __builtin_amdgcn_exp2f(d);
+        s += e;
+        t = fmaf(fmaxf(d, SR_FAR), e, t);
+    }
+    __device__ __forceinline__ void join(float om, float os, float ot) {
+        const float mn = fmaxf(m, om);
+        Soft o{om, os, ot};
+        o.shift_to(mn);
+        shift_to(mn);
+        s += o.s;
+        t += o.t;
+    }
+    __device__ __forceinline__ bool empty() const { return s == 0.f; }
+    __device__ __forceinline__ float entropy(float log_s) const {
+        if (empty()) return 0.f;
+        const float h = log_s - SR_LN2 * t / s;
+        return h < 0.f ? 0.f : h;                         // keeps a NaN
+    }
+};
+
+// The K largest, descending; offered in ascending class order, so that of equal ones the lowest class stays in front.
+template <int K>
+struct Top {
+    float v[K > 0 ? K : 1];
+    int i[K > 0 ? K : 1];
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int j = 0; j < K; ++j) { v[j] = -INFINITY; i[j] = -1; }
+    }
+    __device__ __forceinline__ void offer(float z, int c) {
+        bool g[K > 0 ? K : 1];
+#pragma unroll
+        for (int j = 0; j < K; ++j) g[j] = z > v[j];
+#pragma unroll
+        for (int j = K - 1; j > 0; --j) {
+            i[j] = g[j - 1] ? i[j - 1] : (g[j] ? c : i[j]);
+            v[j] = g[j - 1] ? v[j - 1] : (g[j] ? z : v[j]);
+        }
+        if (K > 0) {
+            i[0] = g[0] ? c : i[0];
+            v[0] = g[0] ? z : v[0];
+        }
+    }
+    // The K largest of the lists of 2^n neighbouring lanes, in every one of them: K times the best head, whose lane moves up.
+    template <int LANES>
+    __device__ __forceinline__ void join_lanes() {
+        Top<K> r;
+#pragma unroll
+        for (int j = 0; j < K; ++j) {
+            float bv = v[0];
+            int bi = i[0];
+#pragma unroll
+            for (int o = 1; o < LANES; o <<= 1) {
+                const float ov = __shfl_xor(bv, o, 64);
+                const int oi = __shfl_xor(bi, o, 64);
+                if (ov > bv || (ov == bv && (unsigned)oi < (unsigned)bi)) { bv = ov; bi = oi; }
+            }
+            const bool mine = bi >= 0 && i[0] == bi;
+#pragma unroll
+            for (int q = 0; q + 1 < K; ++q) {
+                v[q] = mine ? v[q + 1] : v[q];
+                i[q] = mine ? i[q + 1] : i[q];
+            }
+            v[K > 0 ? K - 1 : 0] = mine ? -INFINITY : v[K > 0 ? K - 1 : 0];
+            i[K > 0 ? K - 1 : 0] = mine ? -1 : i[K > 0 ? K - 1 : 0];
+            r.v[j] = bv;
+            r.i[j] = bi;
+        }
+        *this = r;
+    }
+};
+
+// log probability of an alternative: NaN in a row without a distribution, -inf where the row has no such class
+__device__ __forceinline__ float top_log_p(float v, int i, const Soft& a, float log_s) {
+    return a.s != a.s ? a.s : i < 0 ? -INFINITY : (v - a.m) - log_s;
+}
+__device__ __forceinline__ int64_t top_index(int i, const Soft& a) { return a.s != a.s ? -1 : i; }

@@ -22,6 +22,7 @@ import torch.nn as nn
 from . import spec as S
 from .arena import ParamArena
 from .engine import Engine
+from .scores import Scores, _Plan
 
 _LEGACY = re.compile(r'\.(norm|relu|conv)\.(\d)\.')
 
@@ -85,6 +86,7 @@ class _LogitsFn(torch.autograd.Function):
         model, eng = ctx.model, ctx.eng
         if not eng.training:
             raise RuntimeError('DenseASPP: backward needs the forward pass to run in train() mode')
+        eng.pass_id += 1
         prog = eng.prog_up_bwd()
         eng.grad_full.view(grad.shape).copy_(grad)
         # The backward program writes into the flat gradient arena, which the .grad views of a previous train_step
@@ -99,6 +101,44 @@ class _LogitsFn(torch.autograd.Function):
         grads = [model.arena.view(g, n) for n in model._param_names]
         gx = eng.input_gradient().clone() if ctx.needs_input_grad[1] else None
         return (None, gx) + tuple(grads)
+
+
+class _ScoreFn(torch.autograd.Function):
+    """Autograd bridge of ``model.score``: the class scores of the x8-upsampled logits, straight from and to the low-resolution
+    logits of the engine."""
+
+    @staticmethod
+    def forward(ctx, model, x, plan, dropout_masks, generator, *params):
+        eng = model._run_forward(x, dropout_masks=dropout_masks, generator=generator)
+        s, _ = plan.forward(eng.low_logits(), False)
+        ctx.model, ctx.eng, ctx.plan, ctx.pass_id = model, eng, plan, eng.pass_id
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(s.top_class, plan.labels)
+        if s.top_class is not None:
+            ctx.mark_non_differentiable(s.top_class)
+        return tuple(s)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_logp, g_entropy, g_top, _):
+        model, eng = ctx.model, ctx.eng
+        if eng.pass_id != ctx.pass_id:
+            raise RuntimeError('DenseASPP.score: another pass has run since this forward pass and its activations are gone; '
+                               'call backward once, before the next pass')
+        eng.pass_id += 1
+        top_class, _ = ctx.saved_tensors
+        dlow = eng.dlogits.view(eng.B, eng.H2, eng.W2, S.CLS_PAD)[..., :model.spec.n_class].permute(0, 3, 1, 2)
+        ctx.plan.backward(eng.low_logits(), None, None, top_class, g_logp, g_entropy, g_top, out=dlow)
+        # as in _LogitsFn: the arena the .grad views alias keeps its contents
+        held = model._gflat.clone()
+        model._gflat_zero()
+        eng.prog_low_bwd().run()
+        eng._bwd.run()
+        g = model._gflat.clone()
+        model._gflat.copy_(held)
+        grads = [model.arena.view(g, n) for n in model._param_names]
+        gx = eng.input_gradient().clone() if ctx.needs_input_grad[1] else None
+        return (None, gx, None, None, None) + tuple(grads)
 
 
 class DenseASPP(nn.Module):
@@ -414,6 +454,7 @@ class DenseASPP(nn.Module):
         eng = self.engine(B, H, W)
         if refresh:
             self.refresh_weights()
+        eng.pass_id += 1
         eng.set_input(x.detach().to(torch.float32))
         if eng.training:
             eng.draw_dropout(generator=generator, masks=dropout_masks)
@@ -443,6 +484,22 @@ class DenseASPP(nn.Module):
         eng = self._run_forward(x)
         eng.prog_argmax().run()
         return eng.out_argmax.view(eng.B, eng.H, eng.W).clone()
+
+    def score(self, x, labels=None, top_k=0, ignore_index=255, entropy=True, dropout_masks=None, generator=None):
+        """Per-pixel class scores of the full-resolution prediction: Scores(logp, entropy, top_logp, top_class) as
+        scores.label_scores gives them -- log probability of `labels` (int64, N x H x W; 0 at ignore_index), entropy, and the top_k
+        classes with their log probabilities -- computed from the low-resolution logits without the upsampled ones.
+        In train() mode with gradients enabled the result is differentiable with respect to the parameters (and to x), so a
+        loss of one's own trains the network: loss.backward(), then any optimizer."""
+        if x.dim() != 4 or x.shape[1] != 3:
+            raise ValueError('DenseASPP expects an N x 3 x H x W image batch, got %s' % (tuple(x.shape),))
+        if x.shape[2] % 8 or x.shape[3] % 8:
+            raise ValueError('DenseASPP.score: H and W must be multiples of 8, got %d x %d' % tuple(x.shape[2:]))
+        plan = _Plan((x.shape[0], self.spec.n_class, x.shape[2] // 8, x.shape[3] // 8), x.device, labels, top_k, ignore_index, entropy, 8)
+        if torch.is_grad_enabled() and self.training:
+            return Scores(*_ScoreFn.apply(self, x, plan, dropout_masks, generator, *[p for _, p in self.named_parameters()]))
+        eng = self._run_forward(x, dropout_masks=dropout_masks, generator=generator)
+        return plan.forward(eng.low_logits(), False)[0]
 
     def train_step(self, x, labels, ignore_index=255, dropout_masks=None, generator=None, zero_grad=True,
                    refresh=True, reducer=None):

@@ -271,6 +271,8 @@ class Engine:
         self._fwd_loss = None
         self._up_fwd = None
         self._up_bwd = None
+        self._low_bwd = None
+        self.pass_id = 0              # counts the passes that have overwritten the activations
         self._argmax = None
         self._input_grad = None
 
@@ -979,19 +981,29 @@ class Engine:
         """dlogits (fp32 low-res, then bf16 copy) from the full-resolution NCHW fp32 gradient in self.grad_full."""
         sp = self.spec
         self.grad_full = self._zeros(self.B * sp.n_class * self.H * self.W)
-        self.accum_one = torch.zeros(1024, dtype=torch.float32, device=self.device)     # same layout as self.accum
-        self.accum_one[1] = 1.0
         ops = OpList()
         ops.op('memset', src=None, dst=_r(self.dlogits), n=self.dlogits.numel() * 4, value=0, lds=0, ldd=0, rows=0,
                cols=0, dst_cols=0, accumulate=0)
         ops.op('up_bwd', n_img=self.B, h=self.H2, w=self.W2, n_class=sp.n_class, ldl=S.CLS_PAD, logits=_r(self.dlogits),
                out=_r(self.grad_full), argmax=None)
+        self._low_grad_done(ops)
+        return ops
+
+    def build_low_bwd(self):
+        """What the backward pass reads, from a low-resolution logit gradient that is already in self.dlogits."""
+        ops = OpList()
+        self._low_grad_done(ops)
+        return ops
+
+    def _low_grad_done(self, ops):
+        sp = self.spec
+        self.accum_one = torch.zeros(1024, dtype=torch.float32, device=self.device)     # same layout as self.accum
+        self.accum_one[1] = 1.0
         # bf16 copy of the low-res gradient + classifier bias gradient: ce_finalize with the count pinned to 1
         ops.op('ce_finalize', n_img=self.B, h=self.H2, w=self.W2, n_class=sp.n_class, ldl=S.CLS_PAD, logits=None,
                labels=None, ignore_index=-1, dlogits=_r(self.dlogits), accum=_r(self.accum_one), grad_scale=1.0,
                loss=None, dlogits_bf16=None if self.dtype_code else _r(self.dlogits16), lddb=S.CLS_PAD,
                dbias=self.PG('classification.1.bias'))
-        return ops
 
     # ------------------------------------------------------------------ gradient with respect to the input image
     def build_input_grad(self):
@@ -1054,6 +1066,15 @@ class Engine:
         if self._up_bwd is None:
             self._up_bwd = self.backend.compile(self.build_up_bwd())
         return self._up_bwd
+
+    def prog_low_bwd(self):
+        if self._low_bwd is None:
+            self._low_bwd = self.backend.compile(self.build_low_bwd())
+        return self._low_bwd
+
+    def low_logits(self):
+        """The classifier's output as N x n_class x h x w, a view of its NHWC rows."""
+        return self.logits.view(self.B, self.H2, self.W2, S.CLS_PAD)[..., :self.spec.n_class].permute(0, 3, 1, 2)
 
     def prog_argmax(self):
         if self._argmax is None:

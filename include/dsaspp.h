@@ -642,6 +642,8 @@ int dsaspp_adam_step(const dsaspp_adam_desc* d, dsaspp_stream_t stream);
  *      dsaspp_clip_scale: every range times coef in place, rounded once to its type (ranges are left untouched where coef is 1),
  *      norm[0] too; or dsaspp_adam_step_clipped: the Adam update with g * scale * coef; g itself is not written.
  * The three read the partials and nothing but the partials: call 1 with the same ranges first, on the same stream.
+ * dsaspp_clip_grads is 1 and dsaspp_clip_scale in one call (in one kernel where the gradients are few).
+ * Ranges that are written must not overlap: dsaspp_grad_ranges_overlap tells (0 = disjoint, 1 = two of them share memory).
  * dtype of a range: 0 = bf16, 1 = fp32, 2 = fp16. */
 typedef struct dsaspp_grad_range {
     void* p;
@@ -661,6 +663,8 @@ int64_t dsaspp_grad_norm_workspace(const dsaspp_clip_desc* d); /* doubles; -1 on
 int dsaspp_grad_norm_partials(const dsaspp_clip_desc* d, dsaspp_stream_t stream);
 int dsaspp_grad_norm_finish(const dsaspp_clip_desc* d, dsaspp_stream_t stream);
 int dsaspp_clip_scale(const dsaspp_clip_desc* d, dsaspp_stream_t stream);
+int dsaspp_clip_grads(const dsaspp_clip_desc* d, dsaspp_stream_t stream);
+int dsaspp_grad_ranges_overlap(const dsaspp_clip_desc* d);
 /* The update of dsaspp_adam_step with g * c->scale * coef, on any n > 0 elements with no more alignment than their type.  The factors
  * come in double, as an optimizer's host code holds them: 1 - beta2 of a beta2 rounded to fp32 is 1.3e-5 off at 0.999. */
 typedef struct dsaspp_adam_clip_desc {

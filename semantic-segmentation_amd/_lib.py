@@ -141,6 +141,7 @@ OPS = {
     'grad_norm_partials': (None, clip_desc, 'dsaspp_grad_norm_partials'),
     'grad_norm_finish': (None, clip_desc, 'dsaspp_grad_norm_finish'),
     'clip_scale': (None, clip_desc, 'dsaspp_clip_scale'),
+    'clip_grads': (None, clip_desc, 'dsaspp_clip_grads'),
 }
 
 _lib = None
@@ -183,6 +184,7 @@ def load():
                                            ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p]
     lib.dsaspp_stem7_wgrad_workspace_floats.argtypes = [ctypes.c_int32]
     lib.dsaspp_stem7_wgrad_workspace_floats.restype = ctypes.c_int64
+    lib.dsaspp_grad_ranges_overlap.argtypes = [ctypes.POINTER(clip_desc)]
     lib.dsaspp_grad_norm_workspace.argtypes = [ctypes.POINTER(clip_desc)]
     lib.dsaspp_grad_norm_workspace.restype = ctypes.c_int64
     lib.dsaspp_adam_step_clipped.argtypes = [ctypes.POINTER(adam_clip_desc), ctypes.POINTER(clip_desc), ctypes.c_void_p]
@@ -230,6 +232,30 @@ def conv_last_route():
 def check(rc):
     if rc != 0:
         raise DsasppError(load().dsaspp_last_error().decode('utf-8', 'replace'))
+
+
+class _Here:
+    def __enter__(self):
+        pass
+
+    def __exit__(self, *a):
+        pass
+
+
+_HERE = _Here()
+
+
+def on_device(t):
+    """Context in which the device of tensor t is the current one."""
+    import torch
+    index = t.get_device()
+    return _HERE if index == torch.cuda.current_device() else torch.cuda.device(index)
+
+
+def raw_stream(index):
+    """hipStream_t of the current stream of device `index`, as an integer."""
+    import torch
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def exported_symbols():

@@ -7,13 +7,17 @@
 // the coefficient without a third launch, an atomic or a flag.
 #include "elem.h"
 #include <math.h>
+#include <algorithm>
+#include <new>
+#include <utility>
+#include <vector>
 
 namespace {
 
 constexpr int MAX_RANGES = 180;           // ranges that travel in the kernel arguments of one launch (3.6 of 4 KB)
 constexpr int CHUNK = 8192;               // elements of one range that a block takes at a time
-constexpr int MAX_BLOCKS = 2048;          // 8 blocks of 4 waves per CU fill the chip; a block walks several chunks
-constexpr int64_t MAX_ELEMS = (int64_t)CHUNK << 30;
+constexpr int MAX_BLOCKS = 2048;          // 8 blocks of 4 waves per CU fill the chip; a block takes several chunks in a row
+constexpr int64_t MAX_ELEMS = (int64_t)CHUNK << 29;     // chunks of one launch count in 32 bits
 
 struct Group {
     void* p[MAX_RANGES];
@@ -29,6 +33,14 @@ __device__ __forceinline__ int find_range(const Group& g, int chunk) {
         if (g.first[mid] <= chunk) lo = mid; else hi = mid - 1;
     }
     return lo;
+}
+
+// Consecutive chunks of this block: the range is looked up once.  Every block has at least one (the grid has no more blocks).
+struct Share { int first, last; };
+__device__ __forceinline__ Share share_of(int n_chunks) {
+    const int q = n_chunks / (int)gridDim.x, rest = n_chunks - q * (int)gridDim.x, b = blockIdx.x;
+    const int first = b * q + (b < rest ? b : rest);
+    return {first, first + q + (b < rest ? 1 : 0)};
 }
 
 // max that keeps a NaN (fmax drops it)
@@ -57,19 +69,31 @@ __global__ __launch_bounds__(256) void partials_kernel(const Group g, double* ws
         if (MAXNORM) acc[k] = join<true>(acc[k], (double)fabsf(x));
         else acc[k] = __builtin_fma((double)x, (double)x, acc[k]);      // the product is exact: 24 + 24 bits
     };
-    for (int ch = blockIdx.x; ch < n_chunks; ch += gridDim.x) {
-        const int r = find_range(g, ch);
+    const Share sh = share_of(n_chunks);
+    int r = find_range(g, sh.first);
+    for (int ch = sh.first; ch < sh.last; ++ch) {
+        while (ch >= g.first[r + 1]) ++r;
         const int64_t off = (int64_t)(ch - g.first[r]) * CHUNK;
         const int64_t left = g.n[r] - off;
         const int n = left < CHUNK ? (int)left : CHUNK;
         const typename E::T* p = reinterpret_cast<const typename E::T*>(g.p[r]) + off;
-        const int nv = n / E::N;
-        for (int i = threadIdx.x; i < nv; i += 256) {
-            const typename E::V v = *reinterpret_cast<const typename E::V*>(p + (int64_t)i * E::N);
+        constexpr int IT = CHUNK / E::N / 256;                  // loads in flight before the first is used
+        int i = threadIdx.x * E::N;
+        for (; i + ((IT - 1) * 256 + 1) * E::N <= n; i += IT * 256 * E::N) {
+            typename E::V v[IT];
+#pragma unroll
+            for (int it = 0; it < IT; ++it) v[it] = *reinterpret_cast<const typename E::V*>(p + i + it * 256 * E::N);
+#pragma unroll
+            for (int it = 0; it < IT; ++it)
+#pragma unroll
+                for (int k = 0; k < E::N; ++k) take(k & 3, E::up(v[it][k]));
+        }
+        for (; i + E::N <= n; i += 256 * E::N) {
+            const typename E::V v = *reinterpret_cast<const typename E::V*>(p + i);
 #pragma unroll
             for (int k = 0; k < E::N; ++k) take(k & 3, E::up(v[k]));
         }
-        const int t = nv * E::N + (int)threadIdx.x;
+        const int t = n / E::N * E::N + (int)threadIdx.x;
         if (t < n) take(0, E::up(p[t]));                                // fewer than one vector is left
     }
     const double v = join<MAXNORM>(join<MAXNORM>(acc[0], acc[1]), join<MAXNORM>(acc[2], acc[3]));
@@ -112,21 +136,35 @@ __global__ __launch_bounds__(256) void scale_kernel(const Group g, const double*
     const float coef = clip_coef(total, max_norm);
     if (coef == 1.f) return;              // x * 1 is x
     const int n_chunks = g.first[g.n_ranges];
-    for (int ch = blockIdx.x; ch < n_chunks; ch += gridDim.x) {
-        const int r = find_range(g, ch);
+    const Share sh = share_of(n_chunks);
+    int r = find_range(g, sh.last - 1);
+    for (int ch = sh.last - 1; ch >= sh.first; --ch) {                  // backwards: what the norm read last is still in the cache
+        while (ch < g.first[r]) --r;
         const int64_t off = (int64_t)(ch - g.first[r]) * CHUNK;
         const int64_t left = g.n[r] - off;
         const int n = left < CHUNK ? (int)left : CHUNK;
         typename E::T* p = reinterpret_cast<typename E::T*>(g.p[r]) + off;
-        const int nv = n / E::N;
-        for (int i = threadIdx.x; i < nv; i += 256) {
-            typename E::V* q = reinterpret_cast<typename E::V*>(p + (int64_t)i * E::N);
+        constexpr int IT = CHUNK / E::N / 512;
+        int i = threadIdx.x * E::N;
+        for (; i + ((IT - 1) * 256 + 1) * E::N <= n; i += IT * 256 * E::N) {
+            typename E::V v[IT];
+#pragma unroll
+            for (int it = 0; it < IT; ++it) v[it] = *reinterpret_cast<const typename E::V*>(p + i + it * 256 * E::N);
+#pragma unroll
+            for (int it = 0; it < IT; ++it) {
+#pragma unroll
+                for (int k = 0; k < E::N; ++k) v[it][k] = E::down(E::up(v[it][k]) * coef);
+                *reinterpret_cast<typename E::V*>(p + i + it * 256 * E::N) = v[it];
+            }
+        }
+        for (; i + E::N <= n; i += 256 * E::N) {
+            typename E::V* q = reinterpret_cast<typename E::V*>(p + i);
             typename E::V v = *q;
 #pragma unroll
             for (int k = 0; k < E::N; ++k) v[k] = E::down(E::up(v[k]) * coef);
             *q = v;
         }
-        const int t = nv * E::N + (int)threadIdx.x;
+        const int t = n / E::N * E::N + (int)threadIdx.x;
         if (t < n) p[t] = E::down(E::up(p[t]) * coef);
     }
 }
@@ -183,27 +221,39 @@ __global__ __launch_bounds__(256) void adam_clipped_kernel(const AdamArgs d, con
 
 int blocks_for(int64_t chunks) { return (int)(chunks < MAX_BLOCKS ? chunks : MAX_BLOCKS); }
 
-// Calls fn(dtype, group) for every launch the ranges need: up to MAX_RANGES ranges of one type each.
+// Calls fn(dtype, group) for every launch the ranges need: up to MAX_RANGES ranges of one type each.  A range that begins where
+// the one before it ends goes on with it: gradients that are views of one arena.
 template <typename F>
 void for_each_group(const dsaspp_clip_desc& d, F fn) {
     for (int dt = 0; dt < 3; ++dt) {
         Group g;
+        int64_t total = 0;
+        const char* end = nullptr;
         g.n_ranges = 0;
-        g.first[0] = 0;
+        auto flush = [&]() {
+            if (g.n_ranges == 0) return;
+            g.first[0] = 0;
+            for (int i = 0; i < g.n_ranges; ++i) g.first[i + 1] = g.first[i] + (int32_t)((g.n[i] + CHUNK - 1) / CHUNK);
+            fn(dt, g);
+            g.n_ranges = 0;
+            total = 0;
+            end = nullptr;
+        };
         for (int i = 0; i < d.n_ranges; ++i) {
             const dsaspp_grad_range& r = d.ranges[i];
             if (r.dtype != dt) continue;
-            const int64_t chunks = (r.n + CHUNK - 1) / CHUNK;
-            if (g.n_ranges == MAX_RANGES || (g.n_ranges > 0 && g.first[g.n_ranges] + chunks > (1ll << 30))) {
-                fn(dt, g);
-                g.n_ranges = 0;
+            if (total > MAX_ELEMS - r.n) flush();
+            if (g.n_ranges > 0 && end == (const char*)r.p) {
+                g.n[g.n_ranges - 1] += r.n;
+            } else {
+                if (g.n_ranges == MAX_RANGES) flush();
+                g.p[g.n_ranges] = r.p;
+                g.n[g.n_ranges++] = r.n;
             }
-            g.p[g.n_ranges] = r.p;
-            g.n[g.n_ranges] = r.n;
-            g.first[g.n_ranges + 1] = g.first[g.n_ranges] + (int32_t)chunks;
-            ++g.n_ranges;
+            total += r.n;
+            end = (const char*)r.p + r.n * (dt == 1 ? 4 : 2);
         }
-        if (g.n_ranges) fn(dt, g);
+        flush();
     }
 }
 
@@ -235,7 +285,63 @@ int check_ws(const dsaspp_clip_desc* d, const char* who, int64_t* used) {
     return 0;
 }
 
+// Norm and scaling of a few gradients in one block: no second launch, which costs as long as the work.
+constexpr int64_t ONE_BLOCK = 32768;      // elements
+
+template <int DT>
+__global__ __launch_bounds__(1024) void clip_one_kernel(const Group g, int norm_type, float max_norm, float* norm) {
+    typedef Elem<DT> E;
+    __shared__ double lds[16];
+    double acc = 0.0;
+    for (int r = 0; r < g.n_ranges; ++r) {
+        const typename E::T* p = reinterpret_cast<const typename E::T*>(g.p[r]);
+        const int n = (int)g.n[r];
+        for (int i = threadIdx.x; i < n; i += 1024) {
+            const float x = E::up(p[i]);
+            acc = norm_type == 2 ? __builtin_fma((double)x, (double)x, acc) : join<true>(acc, (double)fabsf(x));
+        }
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const double other = __shfl_xor(acc, o, 64);
+        acc = norm_type == 2 ? acc + other : join<true>(acc, other);
+    }
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = acc;
+    __syncthreads();                      // also: every element has been read before any is written
+    acc = lds[0];
+#pragma unroll
+    for (int w = 1; w < 16; ++w) acc = norm_type == 2 ? acc + lds[w] : join<true>(acc, lds[w]);
+    const double total = norm_type == 2 ? sqrt(acc) : acc;
+    if (threadIdx.x == 0) norm[0] = (float)total;
+    const float coef = clip_coef(total, max_norm);
+    if (coef == 1.f) return;
+    for (int r = 0; r < g.n_ranges; ++r) {
+        typename E::T* p = reinterpret_cast<typename E::T*>(g.p[r]);
+        const int n = (int)g.n[r];
+        for (int i = threadIdx.x; i < n; i += 1024) p[i] = E::down(E::up(p[i]) * coef);
+    }
+}
+
 }  // namespace
+
+extern "C" int dsaspp_grad_ranges_overlap(const dsaspp_clip_desc* d) {
+    if (check(d, "grad_ranges_overlap")) return -1;
+    std::vector<std::pair<uintptr_t, uintptr_t>> v;
+    try {
+        v.reserve(d->n_ranges);
+    } catch (const std::bad_alloc&) {
+        dsaspp_set_error("grad_ranges_overlap: out of host memory");
+        return -1;
+    }
+    for (int i = 0; i < d->n_ranges; ++i) {
+        const uintptr_t p = (uintptr_t)d->ranges[i].p;
+        v.emplace_back(p, p + (uintptr_t)d->ranges[i].n * (d->ranges[i].dtype == 1 ? 4 : 2));
+    }
+    std::sort(v.begin(), v.end());
+    for (size_t i = 1; i < v.size(); ++i)
+        if (v[i].first < v[i - 1].second) return 1;
+    return 0;
+}
 
 extern "C" int64_t dsaspp_grad_norm_workspace(const dsaspp_clip_desc* d) {
     if (check(d, "grad_norm_workspace")) return -1;
@@ -284,6 +390,30 @@ extern "C" int dsaspp_clip_scale(const dsaspp_clip_desc* d, dsaspp_stream_t stre
         else hipLaunchKernelGGL(scale_kernel<2>, dim3(nb), dim3(256), 0, s, g, d->ws, (int)used, d->norm_type, d->max_norm, d->norm);
     });
     DS_LAUNCH_CHECK("clip_scale");
+    return 0;
+}
+
+extern "C" int dsaspp_clip_grads(const dsaspp_clip_desc* d, dsaspp_stream_t stream) {
+    int64_t used = 0;
+    if (int rc = check_ws(d, "clip_grads", &used)) return rc;
+    DS_REQUIRE(d->norm && d->scale == 1.f && d->max_norm >= 0.f, "clip_grads: null output, scale other than 1 or negative max_norm");
+    int64_t total = 0;
+    int groups = 0;
+    for_each_group(*d, [&](int, const Group& g) {
+        ++groups;
+        for (int i = 0; i < g.n_ranges; ++i) total += g.n[i] < ONE_BLOCK ? g.n[i] : ONE_BLOCK + 1;
+    });
+    if (groups != 1 || total > ONE_BLOCK) {
+        if (int rc = dsaspp_grad_norm_partials(d, stream)) return rc;
+        return dsaspp_clip_scale(d, stream);
+    }
+    hipStream_t s = (hipStream_t)stream;
+    for_each_group(*d, [&](int dt, const Group& g) {
+        if (dt == 0) hipLaunchKernelGGL(clip_one_kernel<0>, dim3(1), dim3(1024), 0, s, g, d->norm_type, d->max_norm, d->norm);
+        else if (dt == 1) hipLaunchKernelGGL(clip_one_kernel<1>, dim3(1), dim3(1024), 0, s, g, d->norm_type, d->max_norm, d->norm);
+        else hipLaunchKernelGGL(clip_one_kernel<2>, dim3(1), dim3(1024), 0, s, g, d->norm_type, d->max_norm, d->norm);
+    });
+    DS_LAUNCH_CHECK("clip_grads");
     return 0;
 }
 

@@ -17,7 +17,9 @@ for the GPU unless error_if_nonfinite is set.
 """
 import ctypes
 import math
+import operator
 
+import numpy
 import torch
 
 from . import _lib
@@ -29,6 +31,7 @@ def _unwrap(model):
 
 _DTYPE_CODE = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}
 _MAX_PIECES = 1 << 16
+_dtype_of, _requires_grad = operator.attrgetter('dtype'), operator.attrgetter('requires_grad')
 
 
 def _dense_pieces(t):
@@ -51,69 +54,65 @@ def _dense_pieces(t):
 
 
 class _Grads:
-    """The device ranges of a list of gradient tensors, joined where one ends at the start of the next, and the descriptor of
-    the norm kernels over them.  Lives for one call."""
+    """The device ranges of a list of gradient tensors and the descriptor of the norm kernels over them.  Lives for one call.
+
+    A list of hundreds of tensors costs more host time to look at than the kernels take, so every property is read in one
+    pass of C calls over the list, and the ranges travel as one array of (address, elements, type code) words, which is the layout of
+    dsaspp_grad_range.  Joining neighbours and looking for overlaps is the library's."""
 
     def __init__(self, grads, norm_type, in_place, who):
-        if isinstance(grads, torch.Tensor):
-            grads = [grads]
-        self.tensors = grads = list(grads)
         norm_type = float(norm_type)
         if norm_type not in (2.0, math.inf):
             raise ValueError('%s: norm_type must be 2 or inf, got %r' % (who, norm_type))
-        dev = None
-        spans = []
-        for t in grads:
-            if not isinstance(t, torch.Tensor):
-                raise TypeError('%s needs tensors, got %s' % (who, type(t).__name__))
-            code = _DTYPE_CODE.get(t.dtype)
-            if code is None or t.layout is not torch.strided:
-                raise TypeError('%s needs dense float32, bfloat16 or float16 gradients, got %s (%s)' % (who, t.dtype, t.layout))
-            if dev is None:
-                dev = t.device
-            if t.device != dev or not t.is_cuda:
-                raise ValueError('%s: the gradients must be on one GPU, got %s and %s' % (who, dev, t.device))
-            n = t.numel()
-            if n == 0:
-                continue
-            if t.is_contiguous() or (t.dim() == 4 and t.is_contiguous(memory_format=torch.channels_last)):
-                spans.append((code, t.data_ptr(), n))
+        T = torch.Tensor
+        try:
+            devices = set(map(T.get_device, grads))
+            dtypes = set(map(_dtype_of, grads))
+            dense = all(map(T.is_contiguous, grads))
+            if len(devices) != 1 or -1 in devices:
+                raise ValueError('%s: the gradients must be on one GPU, got %s' % (who, ', '.join(sorted({str(t.device) for t in grads}))))
+            for dt in dtypes:
+                if dt not in _DTYPE_CODE:
+                    raise TypeError('%s needs float32, bfloat16 or float16 gradients, got %s' % (who, dt))
+            if len(dtypes) == 1:
+                codes = _DTYPE_CODE[next(iter(dtypes))]
             else:
-                spans.extend((code, p, k) for p, k in _dense_pieces(t))
-        if dev is None:
-            raise ValueError('%s needs at least one gradient' % who)
-        size = (2, 4, 2)
-        if in_place:
-            end = 0
-            for p, e in sorted((p, p + n * size[code]) for code, p, n in spans):
-                if p < end:
-                    raise ValueError('%s: two gradients (or two elements of one) share memory: each would be scaled twice' % who)
-                end = e
-        ranges = []
-        last = None
-        for code, p, n in spans:
-            if last is not None and last[0] == code and p == last[1] + last[2] * size[code]:
-                last[2] += n
+                codes = [_DTYPE_CODE[t.dtype] for t in grads]
+            if dense:
+                ptrs, counts = list(map(T.data_ptr, grads)), list(map(T.numel, grads))
             else:
-                last = [code, p, n]
-                ranges.append(last)
-        self.device = dev
-        self.ranges = (_lib.grad_range * max(len(ranges), 1))()
-        for r, (code, p, n) in zip(self.ranges, ranges):
-            r.p, r.n, r.dtype = p, n, code
-        d = self.desc = _lib.clip_desc()
-        d.ranges, d.n_ranges = ctypes.cast(self.ranges, ctypes.c_void_p), len(ranges)
-        d.norm_type = 2 if norm_type == 2.0 else 0
-        d.scale, d.max_norm = 1.0, 0.0
-        self.lib = _lib.load()
-        need = self.lib.dsaspp_grad_norm_workspace(ctypes.byref(d))
+                ptrs, counts, piece_codes = [], [], []
+                for t in grads:
+                    if t.is_contiguous() or (t.dim() == 4 and t.is_contiguous(memory_format=torch.channels_last)):
+                        pieces = ((t.data_ptr(), t.numel()),)
+                    else:
+                        pieces = _dense_pieces(t) if t.numel() else ()
+                    for p, n in pieces:
+                        ptrs.append(p)
+                        counts.append(n)
+                        piece_codes.append(_DTYPE_CODE[t.dtype])
+                codes = piece_codes
+        except (RuntimeError, NotImplementedError) as e:
+            raise TypeError('%s needs dense gradient tensors: %s' % (who, e)) from None
+        self.words = words = numpy.empty((len(ptrs), 3), dtype=numpy.int64)     # read by the calls below
+        if ptrs:
+            words[:, 0], words[:, 1], words[:, 2] = ptrs, counts, codes
+        if 0 in counts:
+            self.words = words = numpy.ascontiguousarray(words[words[:, 1] != 0])
+        dev = devices.pop()
+        d = self.desc = _lib.clip_desc(words.ctypes.data, len(words), 2 if norm_type == 2.0 else 0, 1.0, 0.0)
+        self.lib = lib = _lib.load()
+        if in_place and lib.dsaspp_grad_ranges_overlap(ctypes.byref(d)) != 0:
+            raise ValueError('%s: two gradients (or two elements of one) share memory: each would be scaled twice' % who)
+        need = lib.dsaspp_grad_norm_workspace(ctypes.byref(d))
         if need < 0:
-            raise _lib.DsasppError(self.lib.dsaspp_last_error().decode())
+            raise _lib.DsasppError(lib.dsaspp_last_error().decode())
         # from the caching allocator for this call: two calls, streams or captured graphs never share a workspace
-        self.ws = torch.empty(need, dtype=torch.float64, device=dev)
-        self.norm = torch.empty((), dtype=torch.float32, device=dev)
+        device = grads[0].device
+        self.ws = torch.empty(need, dtype=torch.float64, device=device)
+        self.norm = torch.empty((), dtype=torch.float32, device=device)
         d.ws, d.ws_len, d.norm = self.ws.data_ptr(), need, self.norm.data_ptr()
-        self.stream = ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
+        self.stream = _lib.raw_stream(dev)
 
     def call(self, name):
         _lib.check(getattr(self.lib, name)(ctypes.byref(self.desc), self.stream))
@@ -121,28 +120,35 @@ class _Grads:
 
 def _written(tensors):
     """Tell autograd that the kernels wrote these tensors, as torch's own in-place operations do."""
-    torch.autograd.graph.increment_version([t for t in tensors if not t.is_inference()])
+    try:
+        torch.autograd.graph.increment_version(tensors)
+    except RuntimeError:                       # tensors made in inference mode have no version
+        torch.autograd.graph.increment_version([t for t in tensors if not t.is_inference()])
+
+
+def _checked(grads, who):
+    """The gradients as a list of GPU tensors."""
+    grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
+    for kind in set(map(type, grads)):
+        if not issubclass(kind, torch.Tensor):
+            raise TypeError('%s needs tensors, got %s' % (who, kind.__name__))
+    if grads and not grads[0].is_cuda:
+        raise ValueError('%s needs gradients on a GPU, got %s' % (who, grads[0].device))
+    return grads
 
 
 def grad_norm(grads, norm_type=2.0):
     """Global norm of a list of gradient tensors (or of one): sqrt of the sum of all squares, or the largest magnitude for
     norm_type=inf, as a 0-dim fp32 tensor on their GPU.  float32, bfloat16 and float16 tensors may be mixed.  The sums are fp64:
     magnitudes whose squares leave the fp32 range count in full, and the same tensors give the same bits each time."""
-    grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
+    grads = _checked(grads, 'grad_norm')
     if not grads:
         return torch.tensor(0.0)
-    with torch.cuda.device(_device_of(grads, 'grad_norm')):
+    with _lib.on_device(grads[0]):
         g = _Grads(grads, norm_type, False, 'grad_norm')
         g.call('dsaspp_grad_norm_partials')
         g.call('dsaspp_grad_norm_finish')
     return g.norm
-
-
-def _device_of(grads, who):
-    for t in grads:
-        if not isinstance(t, torch.Tensor) or not t.is_cuda:
-            raise ValueError('%s needs gradients on a GPU, got %s' % (who, t.device if isinstance(t, torch.Tensor) else type(t).__name__))
-    return grads[0].device
 
 
 def clip_grads_(grads, max_norm, norm_type=2.0, error_if_nonfinite=False):
@@ -150,25 +156,27 @@ def clip_grads_(grads, max_norm, norm_type=2.0, error_if_nonfinite=False):
     return the norm (0-dim fp32 tensor on the GPU).  A NaN norm makes every gradient NaN, as torch's clipping does, unless
     error_if_nonfinite is set: then the call waits for the norm and raises RuntimeError before it writes anything.
     Tensors that share memory are refused."""
-    grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
+    grads = _checked(grads, 'clip_grads_')
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError('clip_grads_: max_norm must be >= 0, got %r' % max_norm)
     if not grads:
         return torch.tensor(0.0)
-    if any(t.requires_grad for t in grads if isinstance(t, torch.Tensor)):
+    if any(map(_requires_grad, grads)):
         raise ValueError('clip_grads_ writes plain gradient tensors in place; a tensor that requires grad is not one (pass p.grad, or '
                          'use clip_grad_norm_ on the parameters)')
-    with torch.cuda.device(_device_of(grads, 'clip_grads_')):
+    with _lib.on_device(grads[0]):
         g = _Grads(grads, norm_type, True, 'clip_grads_')
         g.desc.max_norm = max_norm
-        g.call('dsaspp_grad_norm_partials')
         if error_if_nonfinite:
+            g.call('dsaspp_grad_norm_partials')
             g.call('dsaspp_grad_norm_finish')
             if not math.isfinite(float(g.norm)):
                 raise RuntimeError('the norm of the gradients is not finite (%r): nothing was clipped' % float(g.norm))
-        g.call('dsaspp_clip_scale')
-    _written(g.tensors)
+            g.call('dsaspp_clip_scale')
+        else:
+            g.call('dsaspp_clip_grads')
+    _written(grads)
     return g.norm
 
 
@@ -208,7 +216,7 @@ def adam_update_(param, grad, exp_avg, exp_avg_sq, step, lr=1e-3, betas=(0.9, 0.
         raise ValueError('adam_update_: max_grad_norm must be >= 0, got %r' % (max_grad_norm,))
     if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
         raise ValueError('adam_update_: betas must be in [0, 1), got %r' % (betas,))
-    with torch.cuda.device(param.device):
+    with _lib.on_device(param):
         c = _Grads([grad], norm_type, False, 'adam_update_')
         c.desc.scale, c.desc.max_norm = float(grad_scale), float(max_grad_norm)
         c.call('dsaspp_grad_norm_partials')

@@ -8,6 +8,7 @@
 // contiguous: a group of lanes shares a row and reads 16 bytes per lane) and "planes" (class stride other than 1, NCHW: a lane owns
 // P neighbouring pixels and walks the classes).
 #include "softrow.h"
+#include <stdlib.h>
 
 namespace {
 
@@ -53,7 +54,87 @@ __device__ __forceinline__ void store_stats(float* stats, int64_t row, const Sof
     stats[2 * row + 1] = s.empty() ? INFINITY : log_s;
 }
 
+typedef int64_t i64x2u __attribute__((ext_vector_type(2), aligned(8)));
+// P neighbouring values of a row tensor; np < P only at the end of a row of pixels
+template <int P>
+__device__ __forceinline__ void load_row(const float* p, int np, float (&f)[P]) {
+    if (P == 4 && np == P) {
+        const f32x4u v = *reinterpret_cast<const f32x4u*>(p);
+#pragma unroll
+        for (int k = 0; k < P; ++k) f[k] = v[k & 3];
+    } else {
+#pragma unroll
+        for (int k = 0; k < P; ++k) f[k] = k < np ? p[k] : 0.f;
+    }
+}
+template <int P>
+__device__ __forceinline__ void load_row(const int64_t* p, int np, int64_t (&f)[P]) {
+    if (P == 4 && np == P) {
+        const i64x2u v = *reinterpret_cast<const i64x2u*>(p), w = *reinterpret_cast<const i64x2u*>(p + 2);
+#pragma unroll
+        for (int k = 0; k < P; ++k) f[k] = k < 2 ? v[k & 1] : w[k & 1];
+    } else {
+#pragma unroll
+        for (int k = 0; k < P; ++k) f[k] = k < np ? p[k] : 0;
+    }
+}
+template <int P>
+__device__ __forceinline__ void store_row(float* p, int np, const float (&f)[P]) {
+    if (P == 4 && np == P) {
+        f32x4u v;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = f[k < P ? k : 0];
+        *reinterpret_cast<f32x4u*>(p) = v;
+    } else {
+#pragma unroll
+        for (int k = 0; k < P; ++k)
+            if (k < np) p[k] = f[k];
+    }
+}
+template <int P>
+__device__ __forceinline__ void store_row(int64_t* p, int np, const int64_t (&f)[P]) {
+    if (P == 4 && np == P) {
+        i64x2u v, w;
+        v[0] = f[0]; v[1] = f[1 % P]; w[0] = f[2 % P]; w[1] = f[3 % P];
+        *reinterpret_cast<i64x2u*>(p) = v;
+        *reinterpret_cast<i64x2u*>(p + 2) = w;
+    } else {
+#pragma unroll
+        for (int k = 0; k < P; ++k)
+            if (k < np) p[k] = f[k];
+    }
+}
+template <int P>
+__device__ __forceinline__ void load_labels(const dsaspp_scores_desc& d, int64_t row, int np, int (&label)[P]) {
+    if (!d.labels) {
+#pragma unroll
+        for (int q = 0; q < P; ++q) label[q] = -1;
+        return;
+    }
+    int64_t l[P];
+    load_row<P>(d.labels + row, np, l);
+#pragma unroll
+    for (int q = 0; q < P; ++q) label[q] = l[q] != d.ignore_index && l[q] >= 0 && l[q] < d.n_class ? (int)l[q] : -1;
+}
+
 // ---------------------------------------------------------------- rows: TPR lanes share a row
+// The vector of N classes from c on; returns the class of its first element.  At the end of a row whose length is no multiple of N it
+// is the row's last N classes instead, with those before c (another lane's) at -inf: wide loads for rows of any length >= N.
+template <int DT>
+__device__ __forceinline__ int load_classes(const typename Elem<DT>::T* z, int c, int V, float (&f)[Elem<DT>::N]) {
+    typedef Elem<DT> E;
+    if (V >= E::N) {
+        const int base = c + E::N <= V ? c : V - E::N;
+        const typename E::V v = *reinterpret_cast<const typename E::V*>(z + base);
+#pragma unroll
+        for (int k = 0; k < E::N; ++k) f[k] = base + k >= c ? E::up(v[k]) : -INFINITY;
+        return base;
+    }
+#pragma unroll
+    for (int k = 0; k < E::N; ++k) f[k] = k < V ? E::up(z[k]) : -INFINITY;
+    return 0;
+}
+
 template <int DT, int K, int TPR>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rows_fwd_kernel(const Args a) {
     typedef Elem<DT> E;
@@ -83,21 +164,12 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rows_fwd_kernel(const A
                 top.offer(f[k], c + k);
             }
         };
-        const int full = V / E::N * E::N;
-        for (int c = lane * E::N; c < full; c += TPR * E::N) {
-            const typename E::V v = *reinterpret_cast<const typename E::V*>(z + c);
+        for (int c = lane * E::N; c < V; c += TPR * E::N) {
             float f[E::N];
-#pragma unroll
-            for (int k = 0; k < E::N; ++k) f[k] = E::up(v[k]);
-            take(f, E::N, c);
-        }
-        if (full + lane < V) {            // fewer than E::N <= 8 <= TPR are left
-            const float f = E::up(z[full + lane]);
-            take(&f, 1, full + lane);
+            take(f, E::N, load_classes<DT>(z, c, V, f));
         }
         constexpr int G = TPR < 64 ? TPR : 64;
-#pragma unroll
-        for (int o = 1; o < G; o <<= 1) s.join(__shfl_xor(s.m, o, 64), __shfl_xor(s.s, o, 64), __shfl_xor(s.t, o, 64));
+        s.template join_lanes<G>();
         top.template join_lanes<G>();
         if (TPR > 64) {
             const int wave = threadIdx.x >> 6, wl = threadIdx.x & 63;
@@ -116,8 +188,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rows_fwd_kernel(const A
 #pragma unroll
                 for (int j = 0; j < K; ++j) { top.v[j] = lv[wl][j]; top.i[j] = li[wl][j]; }
             }
-#pragma unroll
-            for (int o = 1; o < WAVES; o <<= 1) s.join(__shfl_xor(s.m, o, 64), __shfl_xor(s.s, o, 64), __shfl_xor(s.t, o, 64));
+            s.template join_lanes<WAVES>();
             top.template join_lanes<WAVES>();
         }
         const float log_s = logf(s.s);
@@ -143,31 +214,27 @@ struct Up {
     float t[K > 0 ? K : 1];
     int label, top[K > 0 ? K : 1];
     bool live;
-    __device__ __forceinline__ void load(const dsaspp_scores_desc& d, int64_t plane, int64_t row, int64_t i0, int64_t rem) {
-        m = d.stats[2 * row];
-        log_s = d.stats[2 * row + 1];
-        label = label_of(d, row);
-        a = d.g_logp && label >= 0 ? d.g_logp[d.g_logp_one ? 0 : row] : 0.f;
-        b = d.g_entropy ? d.g_entropy[d.g_entropy_one ? 0 : row] : 0.f;
-        h = d.g_entropy ? d.entropy[row] : 0.f;
+    // from the statistics, the label and the upstream gradients; g_top and the alternatives follow one by one
+    __device__ __forceinline__ void start(float m_, float log_s_, float h_, int label_, float g_logp, float g_entropy) {
+        m = m_;
+        log_s = log_s_;
+        h = h_;
+        label = label_;
+        a = label >= 0 ? g_logp : 0.f;
+        b = g_entropy;
         A = a;
         live = a != 0.f || b != 0.f;
 #pragma unroll
-        for (int j = 0; j < K; ++j) {
-            t[j] = 0.f;
-            top[j] = -1;
-            if (d.g_top && j < d.top_k) {
-                const int64_t o = (i0 * d.top_k + j) * plane + rem;
-                top[j] = (int)d.top_class[o];
-                const float g = d.g_top[d.g_top_one ? 0 : o];
-                // without alternatives because of a NaN: the gradient is NaN unless nothing flows back
-                t[j] = top[j] >= 0 ? g : (log_s != log_s && g != 0.f) ? log_s : 0.f;
-                A += t[j];
-                live = live || t[j] != 0.f;
-            }
-        }
-        live = live && log_s != INFINITY;      // every class masked out
+        for (int j = 0; j < K; ++j) { t[j] = 0.f; top[j] = -1; }
     }
+    __device__ __forceinline__ void add_top(int j, int64_t cls, float g) {
+        top[j] = (int)cls;
+        // without alternatives because of a NaN: the gradient is NaN unless nothing flows back
+        t[j] = cls >= 0 ? g : (log_s != log_s && g != 0.f) ? log_s : 0.f;
+        A += t[j];
+        live = live || t[j] != 0.f;
+    }
+    __device__ __forceinline__ void finish() { live = live && log_s != INFINITY; }        // +inf: every class masked out
     __device__ __forceinline__ float grad(float z, int c) const {
         const float lp = (z - m) - log_s, p = __builtin_amdgcn_exp2f(lp * SR_LOG2E);
         float g = -p * fmaf(b, fmaxf(lp, SR_FAR) + h, A);
@@ -179,6 +246,63 @@ struct Up {
     }
 };
 
+// For P neighbouring rows; np < P only at the end of a row of pixels (the rest is dead).
+template <int K, int P>
+__device__ __forceinline__ void load_up(const dsaspp_scores_desc& d, int64_t plane, int64_t row, int64_t i0, int64_t rem, int np, Up<K> (&u)[P]) {
+    int label[P];
+    float st[2 * P], h[P], ga[P], gb[P];
+    load_labels<P>(d, row, np, label);
+    if (P == 4 && np == P) {
+        float lo[4], hi[4];
+        load_row<4>(d.stats + 2 * row, 4, lo);
+        load_row<4>(d.stats + 2 * row + 4, 4, hi);
+#pragma unroll
+        for (int k = 0; k < 2 * P; ++k) st[k] = k < 4 ? lo[k & 3] : hi[k & 3];
+    } else {
+#pragma unroll
+        for (int k = 0; k < 2 * P; ++k) st[k] = k < 2 * np ? d.stats[2 * row + k] : 0.f;
+    }
+#pragma unroll
+    for (int q = 0; q < P; ++q) { h[q] = 0.f; ga[q] = 0.f; gb[q] = 0.f; }
+    if (d.g_logp) {
+        if (d.g_logp_one) {
+#pragma unroll
+            for (int q = 0; q < P; ++q) ga[q] = d.g_logp[0];
+        } else {
+            load_row<P>(d.g_logp + row, np, ga);
+        }
+    }
+    if (d.g_entropy) {
+        load_row<P>(d.entropy + row, np, h);
+        if (d.g_entropy_one) {
+#pragma unroll
+            for (int q = 0; q < P; ++q) gb[q] = d.g_entropy[0];
+        } else {
+            load_row<P>(d.g_entropy + row, np, gb);
+        }
+    }
+#pragma unroll
+    for (int q = 0; q < P; ++q) u[q].start(st[2 * q], st[2 * q + 1], h[q], label[q], ga[q], gb[q]);
+#pragma unroll
+    for (int j = 0; j < K; ++j)
+        if (d.g_top && j < d.top_k) {
+            const int64_t at = (i0 * d.top_k + j) * plane + rem;
+            int64_t cls[P];
+            float g[P];
+            load_row<P>(d.top_class + at, np, cls);
+            if (d.g_top_one) {
+#pragma unroll
+                for (int q = 0; q < P; ++q) g[q] = d.g_top[0];
+            } else {
+                load_row<P>(d.g_top + at, np, g);
+            }
+#pragma unroll
+            for (int q = 0; q < P; ++q) u[q].add_top(j, cls[q], g[q]);
+        }
+#pragma unroll
+    for (int q = 0; q < P; ++q) u[q].finish();
+}
+
 template <int DT, int K, int TPR>
 __global__ __launch_bounds__(256) void rows_bwd_kernel(const Args a) {
     typedef Elem<DT> E;
@@ -189,17 +313,23 @@ __global__ __launch_bounds__(256) void rows_bwd_kernel(const Args a) {
         const Row r = row_of(a, row);
         const typename E::T* z = reinterpret_cast<const typename E::T*>(d.logits) + r.off;
         typename E::T* o = reinterpret_cast<typename E::T*>(d.dlogits) + row * V;
-        Up<K> u;
-        u.load(d, a.plane, row, r.i0, r.rem);
-        const int full = V / E::N * E::N;
-        for (int c = lane * E::N; c < full; c += TPR * E::N) {
-            const typename E::V v = *reinterpret_cast<const typename E::V*>(z + c);
-            typename E::V w;
+        Up<K> us[1];
+        load_up<K, 1>(d, a.plane, row, r.i0, r.rem, 1, us);
+        const Up<K>& u = us[0];
+        for (int c = lane * E::N; c < V; c += TPR * E::N) {
+            float f[E::N];
+            const int base = load_classes<DT>(z, c, V, f);
+            if (base == c && V >= E::N) {
+                typename E::V w;
 #pragma unroll
-            for (int k = 0; k < E::N; ++k) w[k] = E::down(u.grad(E::up(v[k]), c + k));
-            *reinterpret_cast<typename E::V*>(o + c) = w;
+                for (int k = 0; k < E::N; ++k) w[k] = E::down(u.grad(f[k], c + k));
+                *reinterpret_cast<typename E::V*>(o + c) = w;
+            } else {
+#pragma unroll
+                for (int k = 0; k < E::N; ++k)
+                    if (base + k >= c && base + k < V) o[base + k] = E::down(u.grad(f[k], base + k));
+            }
         }
-        if (full + lane < V) o[full + lane] = E::down(u.grad(E::up(z[full + lane]), full + lane));
     }
 }
 
@@ -235,8 +365,11 @@ __global__ __launch_bounds__(256) void planes_fwd_kernel(const Args a, const int
         const typename E::T* z = reinterpret_cast<const typename E::T*>(d.logits) + r.off;
         Soft s[P];
         Top<K> top[P];
+        int label[P];
+        float zl[P];
+        load_labels<P>(d, row, np, label);
 #pragma unroll
-        for (int q = 0; q < P; ++q) { s[q].clear(); top[q].clear(); }
+        for (int q = 0; q < P; ++q) { s[q].clear(); top[q].clear(); zl[q] = 0.f; }
         int c = 0;
         for (; c + PU <= V; c += PU) {
             float f[PU][P];
@@ -252,6 +385,7 @@ __global__ __launch_bounds__(256) void planes_fwd_kernel(const Args a, const int
                 for (int u = 0; u < PU; ++u) {
                     s[q].add(f[u][q]);
                     top[q].offer(f[u][q], c + u);
+                    zl[q] = label[q] == c + u ? f[u][q] : zl[q];       // a gather afterwards would touch a line per pixel
                 }
             }
         }
@@ -263,27 +397,40 @@ __global__ __launch_bounds__(256) void planes_fwd_kernel(const Args a, const int
                 if (f[q] > s[q].m) s[q].shift_to(f[q]);
                 s[q].add(f[q]);
                 top[q].offer(f[q], c);
+                zl[q] = label[q] == c ? f[q] : zl[q];
             }
         }
+        float log_s[P], o[P];
 #pragma unroll
-        for (int q = 0; q < P; ++q) {
-            if (q >= np) break;
-            const float log_s = logf(s[q].s);
-            if (d.logp) {
-                const int label = label_of(d, row + q);
-                const float zl = label >= 0 ? E::up(z[label * d.sc + q]) : 0.f;
-                d.logp[row + q] = label_log_p(label, zl, s[q], log_s);
-            }
-            if (d.entropy) d.entropy[row + q] = s[q].entropy(log_s);
-            if (d.stats) store_stats(d.stats, row + q, s[q], log_s);
+        for (int q = 0; q < P; ++q) log_s[q] = logf(s[q].s);
+        if (d.logp) {
 #pragma unroll
-            for (int j = 0; j < K; ++j)
-                if (j < d.top_k) {
-                    const int64_t o = (r.i0 * d.top_k + j) * a.plane + r.rem + q;
-                    d.top_logp[o] = top_log_p(top[q].v[j], top[q].i[j], s[q], log_s);
-                    d.top_class[o] = top_index(top[q].i[j], s[q]);
+            for (int q = 0; q < P; ++q) o[q] = label_log_p(label[q], zl[q], s[q], log_s[q]);
+            store_row<P>(d.logp + row, np, o);
+        }
+        if (d.entropy) {
+#pragma unroll
+            for (int q = 0; q < P; ++q) o[q] = s[q].entropy(log_s[q]);
+            store_row<P>(d.entropy + row, np, o);
+        }
+        if (d.stats) {
+#pragma unroll
+            for (int q = 0; q < P; ++q)
+                if (q < np) store_stats(d.stats, row + q, s[q], log_s[q]);
+        }
+#pragma unroll
+        for (int j = 0; j < K; ++j)
+            if (j < d.top_k) {
+                const int64_t at = (r.i0 * d.top_k + j) * a.plane + r.rem;
+                int64_t ti[P];
+#pragma unroll
+                for (int q = 0; q < P; ++q) {
+                    o[q] = top_log_p(top[q].v[j], top[q].i[j], s[q], log_s[q]);
+                    ti[q] = top_index(top[q].i[j], s[q]);
                 }
-        }
+                store_row<P>(d.top_logp + at, np, o);
+                store_row<P>(d.top_class + at, np, ti);
+            }
     }
 }
 
@@ -300,8 +447,7 @@ __global__ __launch_bounds__(256) void planes_bwd_kernel(const Args a, const int
         const typename E::T* z = reinterpret_cast<const typename E::T*>(d.logits) + r.off;
         typename E::T* o = reinterpret_cast<typename E::T*>(d.dlogits) + r.i0 * V * a.plane + r.rem;
         Up<K> u[P];
-#pragma unroll
-        for (int q = 0; q < P; ++q) u[q].load(d, a.plane, q < np ? row + q : row, r.i0, q < np ? r.rem + q : r.rem);
+        load_up<K, P>(d, a.plane, row, r.i0, r.rem, np, u);
 #pragma unroll PU
         for (int c = 0; c < V; ++c) {
             float f[P];
@@ -369,10 +515,16 @@ void launch_rows_tpr(const Args& a, hipStream_t s) {
 
 template <int DT, int K, bool BWD>
 void launch_rows(const Args& a, hipStream_t s) {
-    const int V = a.d.n_class;
-    if (V <= 64) launch_rows_tpr<DT, K, 8, BWD>(a, s);
-    else if (V <= 1024) launch_rows_tpr<DT, K, 64, BWD>(a, s);
-    else if (V <= 8192 || a.rows >= 1024) launch_rows_tpr<DT, K, 256, BWD>(a, s);
+    static const char* e = getenv("TPR");
+    static const int tpr_env = e ? atoi(e) : 0;
+    const int64_t vecs = (a.d.n_class + Elem<DT>::N - 1) / Elem<DT>::N;
+    int tpr = 4;
+    while (tpr < 1024 && tpr * 4 <= vecs && a.rows * tpr < 256 * 1024) tpr *= 4;
+    if (tpr_env) tpr = tpr_env;
+    if (tpr == 4) launch_rows_tpr<DT, K, 4, BWD>(a, s);
+    else if (tpr == 16) launch_rows_tpr<DT, K, 16, BWD>(a, s);
+    else if (tpr == 64) launch_rows_tpr<DT, K, 64, BWD>(a, s);
+    else if (tpr == 256) launch_rows_tpr<DT, K, 256, BWD>(a, s);
     else launch_rows_tpr<DT, K, 1024, BWD>(a, s);
 }
 

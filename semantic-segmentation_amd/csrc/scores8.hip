@@ -30,12 +30,6 @@ __device__ __forceinline__ float mix(float h, float a, float l, float b) {
     return h * a + l * b;
 }
 
-__device__ __forceinline__ float load_any(const void* p, int64_t i, int dtype) {
-    if (dtype == 1) return reinterpret_cast<const float*>(p)[i];
-    const u16 x = reinterpret_cast<const u16*>(p)[i];
-    return dtype == 0 ? Elem<0>::up(x) : Elem<2>::up(x);
-}
-
 struct Tile {
     int n, ci0, cj0;                                  // image, first cell column and row
     __device__ __forceinline__ Tile(int tile, int tiles_x, int tiles_y) {
@@ -47,115 +41,291 @@ struct Tile {
 };
 
 // The corner pixels of the tile's cells, fp32, CS floats apart; cell (i, j) of the tile has its corners at (j..j+1, i..i+1).
-template <int CS>
-__device__ __forceinline__ void stage(const dsaspp_scores8_desc& d, const Tile& t, float* corner) {
-    const int nc = d.n_class, total = PX * PY * nc;
-    const int64_t base = (int64_t)t.n * d.sn;
-    const bool inner = d.sc == 1;                     // the fastest index of the walk is the contiguous one
-    for (int i = threadIdx.x; i < total; i += 256) {
-        int c, px, py;
-        if (inner) {
-            c = i % nc;
-            const int p = i / nc;
-            px = p % PX; py = p / PX;
-        } else {
-            px = i % PX;
-            const int p = i / PX;
-            py = p % PY; c = p / PY;
-        }
+// Returns the largest magnitude among them, NaN counting as the largest, for the whole block.
+template <int CS, int DT>
+__device__ __forceinline__ unsigned stage_typed(const dsaspp_scores8_desc& d, const Tile& t, float* corner) {
+    typedef Elem<DT> E;
+    const typename E::T* L = reinterpret_cast<const typename E::T*>(d.logits) + (int64_t)t.n * d.sn;
+    const int nc = d.n_class;
+    unsigned big = 0;
+    auto address = [&](int px, int py, int c) {
         const int y = min(max(t.cj0 - 1 + py, 0), d.h - 1), x = min(max(t.ci0 - 1 + px, 0), d.w - 1);
-        corner[(py * PX + px) * CS + c] = load_any(d.logits, base + y * d.sy + x * d.sx + c * d.sc, d.dtype);
+        return L + (y * d.sy + x * d.sx + c * d.sc);
+    };
+    auto keep = [&](int px, int py, int c, float v) {
+        big = max(big, __float_as_uint(v) & 0x7fffffffu);       // ordered as the magnitudes are, NaN above infinity
+        corner[(py * PX + px) * CS + c] = v;
+    };
+    if (d.sc == 1) {                                  // 32 lanes per pixel: the classes are contiguous.  All loads first, then their use
+        constexpr int IT = (PX * PY + 7) / 8;
+        const int c = threadIdx.x & 31, p0 = threadIdx.x >> 5;
+        if (c < nc) {
+            typename E::T v[IT];
+#pragma unroll
+            for (int k = 0; k < IT; ++k) {
+                const int p = min(p0 + 8 * k, PX * PY - 1);       // the last ones twice: the same value to the same place
+                v[k] = *address(p % PX, p / PX, c);
+            }
+#pragma unroll
+            for (int k = 0; k < IT; ++k) {
+                const int p = min(p0 + 8 * k, PX * PY - 1);
+                keep(p % PX, p / PX, c, E::up(v[k]));
+            }
+        }
+    } else {
+        for (int i0 = threadIdx.x; i0 < PX * PY * nc; i0 += 1024) {
+            typename E::T v[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int i = min(i0 + 256 * k, PX * PY * nc - 1), p = i / PX;
+                v[k] = *address(i % PX, p % PY, p / PY);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int i = min(i0 + 256 * k, PX * PY * nc - 1), p = i / PX;
+                keep(i % PX, p % PY, p / PY, E::up(v[k]));
+            }
+        }
     }
-    __syncthreads();
+    return big;
 }
 
-// One output column: which it is, its weights and the LDS addresses of its four corners.
+template <int CS>
+__device__ __forceinline__ float stage(const dsaspp_scores8_desc& d, const Tile& t, float* corner, unsigned* largest) {
+    unsigned big;
+    if (d.dtype == 1) big = stage_typed<CS, 1>(d, t, corner);
+    else if (d.dtype == 0) big = stage_typed<CS, 0>(d, t, corner);
+    else big = stage_typed<CS, 2>(d, t, corner);
+    big = ~lanes_min<64>(~big);
+    if ((threadIdx.x & 63) == 0) largest[threadIdx.x >> 6] = big;
+    __syncthreads();
+    return __uint_as_float(max(max(largest[0], largest[1]), max(largest[2], largest[3])));
+}
+
+// One output column: which it is, its weights, where its four corners are in LDS and the rows of its cell.  A wave is one row of
+// cells, so everything about rows is uniform.
+template <int CS>
 struct Column {
-    int X, cj, py, px;
+    int X, cj, r_begin, r_end;                        // rows 8 cj - 4 + [r_begin, r_end)
     bool ok;
     float lx, hx;
-    int o00, o01, o10, o11;
-    __device__ __forceinline__ Column(const dsaspp_scores8_desc& d, const Tile& t, int cs) {
-        const int lane8 = threadIdx.x & 7;
-        px = (threadIdx.x >> 3) & (TCX - 1);
-        py = threadIdx.x >> 6;
+    int at;                                           // of the upper left corner; the others are one pixel right and one line down
+    int to_x0, to_x1, to_y0, to_y1;                   // where the plain form reads instead, see logit()
+    __device__ __forceinline__ Column(const dsaspp_scores8_desc& d, const Tile& t) {
+        const int lane8 = threadIdx.x & 7, px = (threadIdx.x >> 3) & (TCX - 1), py = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         cj = t.cj0 + py;
         X = 8 * (t.ci0 + px) - 4 + lane8;
         ok = cj <= d.h && X >= 0 && X < 8 * d.w;
+        r_begin = cj == 0 ? 4 : 0;
+        r_end = cj == d.h ? 4 : 8;
         int x0, x1;
         src_index(max(X, 0), d.w, x0, x1, lx);
         hx = 1.f - lx;
-        // left of the first pixel's centre the first corner is the pixel itself: LDS column 1 of the first tile, as column 0
-        const int c0 = min(max(x0 - (t.ci0 - 1), 0), PX - 1), c1 = min(max(x1 - (t.ci0 - 1), 0), PX - 1);
-        int y0, y1;
-        float l;
-        src_index(max(8 * cj - 4, 0), d.h, y0, y1, l);
-        const int r0 = min(max(y0 - (t.cj0 - 1), 0), PY - 1), r1 = min(max(y1 - (t.cj0 - 1), 0), PY - 1);
-        o00 = (r0 * PX + c0) * cs; o01 = (r0 * PX + c1) * cs;
-        o10 = (r1 * PX + c0) * cs; o11 = (r1 * PX + c1) * cs;
+        at = (py * PX + px) * CS;
+        // Left of the first pixel's centre (and above it) torch reads pixels 0 and 1 with weights 1 and 0, the tile holds pixel 0 twice: the
+        // same sum unless pixel 1 is not finite.
+        to_x0 = x0 - (t.ci0 - 1 + px) > 0 ? CS : 0;
+        to_x1 = (min(px + 1 + (x0 - (t.ci0 - 1 + px) > 0 && x1 > x0), PX - 1) - px) * CS;
+        const int down = cj == 0 ? 1 : 0;
+        to_y0 = down * PX * CS;
+        to_y1 = (1 + (down && d.h > 1 ? 1 : 0)) * PX * CS;
+    }
+    // weight of the second corner row: (2 r + 1) / 16, but 0 above the first pixel's centre (exact in fp32 either way)
+    __device__ __forceinline__ float ly(int r) const { return cj == 0 ? 0.f : 0.125f * (float)r + 0.0625f; }
+    // the interpolated logit of one class, every product and sum rounded by itself
+    __device__ __forceinline__ float logit(const float* corner, int c, float hy, float ly) const {
+        const float* p = corner + at + c;
+        return mix(hy, mix(hx, p[0], lx, p[CS]), ly, mix(hx, p[PX * CS], lx, p[PX * CS + CS]));
+    }
+    // the same from the very pixels that torch reads, for logits that may be infinite or NaN
+    __device__ __forceinline__ float plain_logit(const float* corner, int c, float hy, float ly) const {
+        const float* p = corner + at + c;
+        return mix(hy, mix(hx, p[to_y0 + to_x0], lx, p[to_y0 + to_x1]), ly, mix(hx, p[to_y1 + to_x0], lx, p[to_y1 + to_x1]));
+    }
+};
+
+// The short form of a column's arithmetic, for columns of tame logits whose two corner rows are alike enough.
+//
+// With M_i = max r_i, x0 = (r0 - M0) log2 e and dx = (r1 - M1) log2 e - x0 the logit of class c in output row r is
+//   (z - up) log2 e = x(r) = x0 + ly(r) dx,   up = hy M0 + ly M1,
+// at most 0 and linear in r, so its exponential is a geometric sequence down the 8 rows of a cell: e(r + 1) = e(r) 2^(dx / 8), one
+// multiplication where an interpolation, a subtraction and an exponential (four issue slots) would be.  It asks for |dx| <= 48: then the
+// sum of a row is at least 2^-48, and a term that starts below the normal range (2^-126) ends below 2^-78 and does not count.
+// A step adds at most 3 half-steps of relative error (the factor's and the product's), seven of them 21; x0 and dx carry the roundings of
+// R = max |r_i|: below 15 R half-steps together in a logarithm.
+// Columns of logits from 1e5 on, and of -inf and NaN, take the plain form.
+constexpr float ALIKE = 48.f, TAME = 1.0e5f;
+constexpr float PAD = -1.0e6f;            // x of the classes past the last one: below that of any tame logit
+
+template <int NC>
+struct Chain {
+    float x0[NC], dx[NC], q[NC], e[NC];
+    float M0, M1;
+    // from the four corners; classes from nc on get exponentials of 0.  Returns whether the short form holds for this lane.
+    template <bool EXACT, int CS>
+    __device__ __forceinline__ bool start(const Column<CS>& col, const float* corner, int nc) {
+        const float* p = corner + col.at;
+        M0 = M1 = -FLT_MAX;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            x0[c] = fmaf(col.lx, p[CS + c], col.hx * p[c]);
+            dx[c] = fmaf(col.lx, p[PX * CS + CS + c], col.hx * p[PX * CS + c]);
+            if (EXACT || c < nc) { M0 = fmaxf(M0, x0[c]); M1 = fmaxf(M1, dx[c]); }
+        }
+        const float m0 = M0 * SR_LOG2E, m1 = M1 * SR_LOG2E, ly = col.ly(col.r_begin);
+        float far = 0.f;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const bool real = EXACT || c < nc;
+            x0[c] = real ? fmaf(x0[c], SR_LOG2E, -m0) : PAD;
+            dx[c] = real && col.cj != 0 ? fmaf(dx[c], SR_LOG2E, -m1) - x0[c] : 0.f;      // the topmost cells have ly = 0 throughout
+            far = fmaxf(far, fabsf(dx[c]));
+            q[c] = __builtin_amdgcn_exp2f(0.125f * dx[c]);
+            e[c] = __builtin_amdgcn_exp2f(fmaf(ly, dx[c], x0[c]));
+        }
+        return far <= ALIKE;
+    }
+    __device__ __forceinline__ float x(int c, float ly) const { return fmaf(ly, dx[c], x0[c]); }
+};
+
+// The K largest of a pixel in the short form.  A key is x with its five lowest bits replaced by the class, so that keeping K + 1
+// keys in order is K + 1 instructions per class (one max, K medians of three) where values and classes apart take 4 K - 1.  Where
+// two neighbours among them are closer than the roundings of x and of the key, the pixel's logits are offered again, exactly.
+// The instructions themselves: the compiler's forms first quieten a key, whose bits might be a signalling NaN for all it knows.
+__device__ __forceinline__ float med3(float a, float b, float c) {
+    float r;
+    asm("v_med3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+__device__ __forceinline__ float larger(float a, float b) {
+    float r;
+    asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+    return r;
+}
+
+template <int K>
+struct Keys {
+    float v[K + 1];
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int j = 0; j <= K; ++j) v[j] = -FLT_MAX;
+    }
+    __device__ __forceinline__ void offer(float x, int c) {
+        const float k = __uint_as_float((__float_as_uint(x) & ~31u) | (unsigned)c);
+#pragma unroll
+        for (int j = K; j > 0; --j) v[j] = med3(v[j - 1], v[j], k);
+        v[0] = larger(v[0], k);
+    }
+    __device__ __forceinline__ int cls(int j) const { return (int)(__float_as_uint(v[j]) & 31u); }
+    // R half-steps of the two x (15 each and as many again, in log2 units 1.44 times that), 2^-18 for the two keys' missing bits, and
+    // something above the class bits of an x of 0 (denormal) where R is 0
+    __device__ __forceinline__ bool unclear(int k, float R) const {
+        const float near = fmaf(R, 96.f * 0x1p-24f, 1.0e-30f);
+        int u = 0;                        // no short circuit: it would put each median into a block of its own, with every key kept for it
+#pragma unroll
+        for (int j = 0; j < K; ++j) u |= (int)(v[j] - v[j + 1] <= fmaf(fabsf(v[j + 1]), 0x1p-18f, near)) & (int)(j < k);
+        return u != 0;
     }
 };
 
 template <int NC, bool EXACT, int K>
-__global__ __launch_bounds__(256) void scores8_fwd_kernel(const dsaspp_scores8_desc d, const int tiles_x, const int tiles_y) {
+__global__ __launch_bounds__(256, NC <= 19 ? (K == 0 ? 4 : 3) : 1) void scores8_fwd_kernel(const dsaspp_scores8_desc d, const int tiles_x,
+                                                                                            const int tiles_y) {
     constexpr int CS = NC | 1;
     __shared__ float corner[PX * PY * CS];
-    const Tile tl(blockIdx.x, tiles_x, tiles_y);
-    stage<CS>(d, tl, corner);
-    const Column q(d, tl, CS);
-    if (!q.ok) return;
-    const int nc = EXACT ? NC : d.n_class, H = 8 * d.h, W = 8 * d.w;
-    float r0[NC], r1[NC];
-#pragma unroll
-    for (int c = 0; c < NC; ++c) {
-        r0[c] = mix(q.hx, corner[q.o00 + c], q.lx, corner[q.o01 + c]);
-        r1[c] = mix(q.hx, corner[q.o10 + c], q.lx, corner[q.o11 + c]);
+    __shared__ unsigned largest[4];
+    const Tile tl(xcd_remap(blockIdx.x, gridDim.x), tiles_x, tiles_y);
+    const Column<CS> q(d, tl);
+    const int nc = EXACT ? NC : d.n_class, W = 8 * d.w;
+    const int64_t plane = 64ll * d.h * d.w;
+    const unsigned X = q.X;               // row bases are uniform, lanes differ in X alone
+    int64_t at = tl.n * plane + (int64_t)(8 * q.cj - 4 + q.r_begin) * W;
+    int64_t next = -1, after = -1;        // labels, two rows ahead; a cell has 4 or 8 rows
+    if (q.ok && d.logp) {
+        next = (d.labels + at)[X];
+        after = (d.labels + at + W)[X];
     }
-    const int64_t image = (int64_t)tl.n * H * W;
-    for (int r = 0; r < 8; ++r) {
-        const int Y = 8 * q.cj - 4 + r;
-        if (Y < 0 || Y >= H) continue;
-        int y0, y1;
-        float ly;
-        src_index(Y, d.h, y0, y1, ly);
-        const float hy = 1.f - ly;
-        float z[NC];
-        Top<K> top;
-        top.clear();
-        Soft s;
-        s.clear();
+    const float R = stage<CS>(d, tl, corner, largest);
+    if (!q.ok) return;
+    Chain<NC> ch;
+    const bool alike = ch.template start<EXACT>(q, corner, nc);
+    const bool brief = R < TAME && __all(alike);
+#pragma unroll 1
+    for (int r = q.r_begin; r < q.r_end; ++r, at += W) {
+        const float ly = q.ly(r), hy = 1.f - ly;
+        const int64_t l = next;
+        next = after;
+        if (d.logp && r + 2 < q.r_end) after = (d.labels + at + 2 * W)[X];
+        const int label = d.logp && l != d.ignore_index && l >= 0 && l < nc ? (int)l : -1;
+        int top_i[K > 0 ? K : 1];
+        float logp, h, top_lp[K > 0 ? K : 1];
+        if (brief) {
+            float s = 0.f, t = 0.f;
+            Keys<K> keys;
+            if (K > 0) keys.clear();
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            z[c] = mix(hy, r0[c], ly, r1[c]);
-            if (!EXACT) z[c] = c < nc ? z[c] : -INFINITY;
-            s.m = fmaxf(s.m, z[c]);
-            top.offer(z[c], c);
-        }
+            for (int c = 0; c < NC; ++c) {
+                const float x = ch.x(c, ly);
+                s += ch.e[c];
+                t = fmaf(x, ch.e[c], t);
+                if (K > 0) keys.offer(x, c);
+                ch.e[c] *= ch.q[c];
+            }
+            const float log2_s = __builtin_amdgcn_logf(s), up = mix(hy, ch.M0, ly, ch.M1);
+            logp = label < 0 ? 0.f : SR_LN2 * ((q.logit(corner, max(label, 0), hy, ly) - up) * SR_LOG2E - log2_s);
+            h = fmaxf(SR_LN2 * (log2_s - t * __builtin_amdgcn_rcpf(s)), 0.f);
+            if (K > 0) {
 #pragma unroll
-        for (int c = 0; c < NC; ++c) s.add(z[c]);
-        const float log_s = logf(s.s);
-        const int64_t pix = (int64_t)Y * W + q.X;
-        if (d.logp) {
-            const int64_t l = d.labels[image + pix];
-            const bool has = l != d.ignore_index && l >= 0 && l < nc;
-            const int lc = has ? (int)l : 0;
-            const float a = mix(q.hx, corner[q.o00 + lc], q.lx, corner[q.o01 + lc]);
-            const float b = mix(q.hx, corner[q.o10 + lc], q.lx, corner[q.o11 + lc]);
-            d.logp[image + pix] = !has ? 0.f : s.empty() ? -INFINITY : (mix(hy, a, ly, b) - s.m) - log_s;
+                for (int j = 0; j < K; ++j) top_i[j] = keys.cls(j);
+                if (keys.unclear(d.top_k, R)) {
+                    Top<K> top;
+                    top.clear();
+#pragma unroll 1
+                    for (int c = 0; c < nc; ++c) top.offer(q.logit(corner, c, hy, ly), c);
+#pragma unroll
+                    for (int j = 0; j < K; ++j) top_i[j] = top.i[j];
+                }
+#pragma unroll
+                for (int j = 0; j < K; ++j)
+                    if (j < d.top_k) top_lp[j] = SR_LN2 * ((q.logit(corner, top_i[j], hy, ly) - up) * SR_LOG2E - log2_s);
+            }
+        } else {
+            Top<K> top;
+            Soft s;
+            top.clear();
+            s.clear();
+#pragma unroll 1
+            for (int c = 0; c < nc; ++c) {
+                const float z = q.plain_logit(corner, c, hy, ly);
+                s.m = fmaxf(s.m, z);
+                top.offer(z, c);
+            }
+#pragma unroll 1
+            for (int c = 0; c < nc; ++c) s.add(q.plain_logit(corner, c, hy, ly));
+            const float log_s = logf(s.s);
+            logp = label < 0 ? 0.f : s.empty() ? -INFINITY : (q.plain_logit(corner, label, hy, ly) - s.m) - log_s;
+            h = s.entropy(log_s);
+#pragma unroll
+            for (int j = 0; j < K; ++j) {
+                top_lp[j] = top_log_p(top.v[j], top.i[j], s, log_s);
+                top_i[j] = (int)top_index(top.i[j], s);
+            }
         }
-        if (d.entropy) d.entropy[image + pix] = s.entropy(log_s);
+        if (d.logp) (d.logp + at)[X] = logp;
+        if (d.entropy) (d.entropy + at)[X] = h;
 #pragma unroll
         for (int j = 0; j < K; ++j)
             if (j < d.top_k) {
-                const int64_t o = ((int64_t)tl.n * d.top_k + j) * H * W + pix;
-                d.top_logp[o] = top_log_p(top.v[j], top.i[j], s, log_s);
-                d.top_class[o] = top_index(top.i[j], s);
+                const int64_t o = at + ((int64_t)tl.n * (d.top_k - 1) + j) * plane;
+                (d.top_logp + o)[X] = top_lp[j];
+                (d.top_class + o)[X] = top_i[j];
             }
     }
 }
 
 __device__ __forceinline__ float row8_sum(float v) {
     // sum over the 8 lanes of a cell (an aligned 8-lane group inside a DPP row), result in every lane
+    asm("" : "+v"(v));                    // the product by itself: folded into the first sum it keeps the swizzle out of the addition
     int x = __float_as_int(v);
     v += __int_as_float(__builtin_amdgcn_update_dpp(0, x, 0xB1, 0xF, 0xF, true));    // quad_perm [1,0,3,2]
     x = __float_as_int(v);
@@ -165,100 +335,121 @@ __device__ __forceinline__ float row8_sum(float v) {
     return v;
 }
 
-// HB: an upstream gradient of the entropy is there.  Per pixel and class  dz = 2^d (k0 + k1 d)  with d = (z - m) log2 e and per-pixel
-// k0, k1; what falls on the label and on the alternatives is added to lane-private LDS columns instead of being selected by class.
+// HB: an upstream gradient of the entropy is there.  Per pixel and class  dz = e (k0 + k1 x)  with e = 2^x, x = (z - up) log2 e for
+// any reference up, and per-pixel k0, k1; what falls on the label and on the alternatives is added to lane-private LDS columns instead of
+// being selected by class.
 template <int NC, bool EXACT, bool HB>
-__global__ __launch_bounds__(256) void scores8_bwd_kernel(const dsaspp_scores8_desc d, const int tiles_x, const int tiles_y) {
+__global__ __launch_bounds__(256, NC <= 19 ? 3 : 1) void scores8_bwd_kernel(const dsaspp_scores8_desc d, const int tiles_x, const int tiles_y) {
     constexpr int CS = NC | 1, CELLS = TCX * TCY, KS = CELLS * CS;
     __shared__ float corner[PX * PY * CS];
     __shared__ float oh[2 * NC * 256];                // [corner row][class][lane]
     __shared__ float ct[4 * KS];                      // [corner][cell][class]
-    const int tid = threadIdx.x, nc = EXACT ? NC : d.n_class, H = 8 * d.h, W = 8 * d.w;
-    const Tile tl(blockIdx.x, tiles_x, tiles_y);
+    __shared__ unsigned largest[4];
+    const int tid = threadIdx.x, nc = EXACT ? NC : d.n_class, W = 8 * d.w;
+    const int tile = xcd_remap(blockIdx.x, gridDim.x);
+    const Tile tl(tile, tiles_x, tiles_y);
 #pragma unroll
     for (int c = 0; c < 2 * NC; ++c) oh[c * 256 + tid] = 0.f;
-    stage<CS>(d, tl, corner);
-    const Column q(d, tl, CS);
+    const Column<CS> q(d, tl);
+    const float R = stage<CS>(d, tl, corner, largest);
     float g0[NC], g1[NC];
 #pragma unroll
     for (int c = 0; c < NC; ++c) { g0[c] = 0.f; g1[c] = 0.f; }
     if (q.ok) {
-        float r0[NC], r1[NC];
-#pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            r0[c] = mix(q.hx, corner[q.o00 + c], q.lx, corner[q.o01 + c]);
-            r1[c] = mix(q.hx, corner[q.o10 + c], q.lx, corner[q.o11 + c]);
-        }
-        const int64_t image = (int64_t)tl.n * H * W;
-        for (int r = 0; r < 8; ++r) {
-            const int Y = 8 * q.cj - 4 + r;
-            if (Y < 0 || Y >= H) continue;
-            int y0, y1;
-            float ly;
-            src_index(Y, d.h, y0, y1, ly);
-            const float hy = 1.f - ly;
-            const int64_t pix = (int64_t)Y * W + q.X;
-            const float b = HB ? d.g_entropy[d.g_entropy_one ? 0 : image + pix] : 0.f;
-            float a = 0.f, A;
-            int label = -1;
-            if (d.g_logp) {
-                const int64_t l = d.labels[image + pix];
-                if (l != d.ignore_index && l >= 0 && l < nc) {
-                    label = (int)l;
-                    a = d.g_logp[d.g_logp_one ? 0 : image + pix];
-                }
-            }
-            A = a;
+        const int64_t plane = 64ll * d.h * d.w;
+        const unsigned X = q.X;           // row bases are uniform, lanes differ in X alone
+        int64_t at = tl.n * plane + (int64_t)(8 * q.cj - 4 + q.r_begin) * W;
+        Chain<NC> ch;
+        const bool alike = ch.template start<EXACT>(q, corner, nc);
+        const bool brief = R < TAME && __all(alike);
+        struct In { int64_t l; float a, b; };
+        auto load = [&](int64_t p) {
+            In v;
+            v.l = d.g_logp ? (d.labels + p)[X] : -1;
+            v.a = d.g_logp ? (d.g_logp_one ? d.g_logp[0] : (d.g_logp + p)[X]) : 0.f;
+            v.b = HB ? (d.g_entropy_one ? d.g_entropy[0] : (d.g_entropy + p)[X]) : 0.f;
+            return v;
+        };
+        In next = load(at);
+#pragma unroll 1
+        for (int r = q.r_begin; r < q.r_end; ++r, at += W) {
+            const float ly = q.ly(r), hy = 1.f - ly;
+            const In in = next;
+            if (r + 1 < q.r_end) next = load(at + W);         // on its way while this row is worked out
+            const int label = d.g_logp && in.l != d.ignore_index && in.l >= 0 && in.l < nc ? (int)in.l : -1;
+            const float a = label >= 0 ? in.a : 0.f, b = in.b;
+            float A = a;
             bool live = a != 0.f || b != 0.f;
             if (d.g_top)
                 for (int j = 0; j < d.top_k; ++j) {
-                    const int64_t o = ((int64_t)tl.n * d.top_k + j) * H * W + pix;
-                    const float g = d.g_top[d.g_top_one ? 0 : o];
+                    const int64_t o = at + ((int64_t)tl.n * (d.top_k - 1) + j) * plane;
+                    const float g = d.g_top_one ? d.g_top[0] : (d.g_top + o)[X];
                     live = live || g != 0.f;
-                    if (d.top_class[o] >= 0) A += g;
+                    if ((d.top_class + o)[X] >= 0) A += g;
                 }
-            if (!live) continue;
-            float z[NC];
-            Soft s;
-            s.clear();
+            // the label's sums are read now and written back after the row's arithmetic
+            float* const o0 = oh + max(label, 0) * 256 + tid;
+            const float w0 = o0[0], w1 = o0[NC * 256];
+            if (brief) {
+                float s = 0.f, t = 0.f;
 #pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                z[c] = mix(hy, r0[c], ly, r1[c]);
-                if (!EXACT) z[c] = c < nc ? z[c] : -INFINITY;
-                s.m = fmaxf(s.m, z[c]);
-            }
-            float e[NC];
+                for (int c = 0; c < NC; ++c) {
+                    s += ch.e[c];
+                    if (HB) t = fmaf(ch.x(c, ly), ch.e[c], t);
+                }
+                float ly2 = ly;                       // x is formed again below: kept, it would cost a register per class and spill
+                asm("" : "+v"(ly2));
+                // log_p + H = (x ln2 - log s) + (log s - ln2 t / s) = ln2 (x - t / s)
+                const float inv = live ? 1.f / s : 0.f;
+                const float k1 = HB ? -b * SR_LN2 * inv : 0.f;
+                const float k0 = HB ? -A * inv - k1 * (t * inv) : -A * inv;
+                const float a0 = hy * k0, a1 = ly * k0;
 #pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                z[c] = (z[c] - s.m) * SR_LOG2E;
-                e[c] = __builtin_amdgcn_exp2f(z[c]);
-                s.s += e[c];
-                if (HB) {
-                    z[c] = fmaxf(z[c], SR_FAR);
-                    s.t = fmaf(z[c], e[c], s.t);
+                for (int c = 0; c < NC; ++c) {
+                    if (HB) {
+                        const float g = ch.e[c] * fmaf(k1, ch.x(c, ly2), k0);
+                        g0[c] = fmaf(hy, g, g0[c]);
+                        g1[c] = fmaf(ly, g, g1[c]);
+                    } else {
+                        g0[c] = fmaf(a0, ch.e[c], g0[c]);
+                        g1[c] = fmaf(a1, ch.e[c], g1[c]);
+                    }
+                    ch.e[c] *= ch.q[c];
+                }
+                if (!live) continue;
+            } else {
+                if (!live) continue;
+                Soft s;
+                s.clear();
+#pragma unroll 1
+                for (int c = 0; c < nc; ++c) s.m = fmaxf(s.m, q.plain_logit(corner, c, hy, ly));
+    #pragma unroll 1
+            for (int c = 0; c < nc; ++c) s.add(q.plain_logit(corner, c, hy, ly));
+                if (s.empty()) continue;              // every class masked out
+                const float inv = 1.f / s.s, k1 = HB ? -b * SR_LN2 * inv : 0.f, k0 = HB ? -A * inv - k1 * (s.t * inv) : -A * inv;
+#pragma unroll 1
+                for (int c = 0; c < nc; ++c) {        // into the lane's own column, as the label below: no register is indexed
+                    const float x = (q.plain_logit(corner, c, hy, ly) - s.m) * SR_LOG2E;
+                    const float g = __builtin_amdgcn_exp2f(x) * fmaf(k1, fmaxf(x, SR_FAR), k0);
+                    oh[c * 256 + tid] += hy * g;
+                    oh[(NC + c) * 256 + tid] += ly * g;
                 }
             }
-            if (s.empty()) continue;                  // every class masked out
-            const float inv = 1.f / s.s;
-            // log_p + H = (d ln2 - log s) + (log s - ln2 t / s) = ln2 (d - t / s)
-            const float k1 = HB ? -b * SR_LN2 * inv : 0.f;
-            const float k0 = HB ? -A * inv - k1 * (s.t * inv) : -A * inv;
-#pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                const float g = HB ? e[c] * fmaf(k1, z[c], k0) : e[c] * k0;
-                g0[c] = fmaf(hy, g, g0[c]);
-                g1[c] = fmaf(ly, g, g1[c]);
-            }
-            if (label >= 0) {
-                oh[label * 256 + tid] += a * hy;
-                oh[(NC + label) * 256 + tid] += a * ly;
+            if (brief) {
+                if (label >= 0) {
+                    o0[0] = fmaf(a, hy, w0);
+                    o0[NC * 256] = fmaf(a, ly, w1);
+                }
+            } else if (label >= 0) {                  // the loop above wrote the same columns
+                o0[0] += a * hy;
+                o0[NC * 256] += a * ly;
             }
             if (d.g_top)
                 for (int j = 0; j < d.top_k; ++j) {
-                    const int64_t o = ((int64_t)tl.n * d.top_k + j) * H * W + pix;
-                    const int64_t tc = d.top_class[o];
+                    const int64_t o = at + ((int64_t)tl.n * (d.top_k - 1) + j) * plane;
+                    const int64_t tc = (d.top_class + o)[X];
                     if (tc >= 0 && tc < nc) {
-                        const float g = d.g_top[d.g_top_one ? 0 : o];
+                        const float g = d.g_top_one ? d.g_top[0] : (d.g_top + o)[X];
                         oh[(int)tc * 256 + tid] += g * hy;
                         oh[(NC + (int)tc) * 256 + tid] += g * ly;
                     }
@@ -285,7 +476,7 @@ __global__ __launch_bounds__(256) void scores8_bwd_kernel(const dsaspp_scores8_d
     }
     __syncthreads();
     // corner pixel (py, px) of the tile is corner 00 of cell (py, px), 01 of (py, px-1), 10 of (py-1, px), 11 of (py-1, px-1)
-    float* out = d.ws + (int64_t)blockIdx.x * (PX * PY) * nc;
+    float* out = d.ws + (int64_t)tile * (PX * PY) * nc;
     for (int i = tid; i < PX * PY * nc; i += 256) {
         const int c = i % nc, p = i / nc, py = p / PX, px = p - py * PX;
         float v = 0.f;
@@ -297,47 +488,61 @@ __global__ __launch_bounds__(256) void scores8_bwd_kernel(const dsaspp_scores8_d
     }
 }
 
-// Positions along one axis whose sums belong to source pixel i of n: (tile, place in the tile), at most 6.  A cell stands for the
-// pixels before clamping; what falls on -1 or n belongs to the border pixel.
+// Positions along one axis, counted before clamping (pixel i is position i + 1, what lies beyond the border falls on the border pixel),
+// and the tiles that hold a position: tile b has positions b TC .. (b + 1) TC.
+struct Span {
+    int first, last;
+    __device__ __forceinline__ Span(int i, int n) : first(i == 0 ? 0 : i + 1), last(i == n - 1 ? n + 1 : i + 1) {}
+};
 template <int TC>
-__device__ __forceinline__ int places(int i, int n, int tiles, int (&tile)[6], int (&at)[6]) {
-    int k = 0;
-#pragma unroll
-    for (int e = -1; e <= 1; ++e) {                   // e = 0: the pixel itself; -1, 1: beyond the border
-        if ((e < 0 && i != 0) || (e > 0 && i != n - 1)) continue;
-        const int u = i + e + 1, b = u / TC, o = u - b * TC;
-        if (b < tiles) { tile[k] = b; at[k] = o; ++k; }
-        if (o == 0 && b > 0) { tile[k] = b - 1; at[k] = TC; ++k; }
-    }
-    return k;
-}
+__device__ __forceinline__ int first_tile(int u) { return u > 0 ? (u - 1) / TC : 0; }
 
-__global__ __launch_bounds__(256) void scores8_gather_kernel(const dsaspp_scores8_desc d, const int tiles_x, const int tiles_y, const int64_t total) {
+// One thread per class of a source pixel in GL lines, whose loads are all on their way before the first is added; classes fastest (as
+// the workspace has them) or, for planes, pixels fastest.
+constexpr int GL = 4;
+__global__ __launch_bounds__(256) void scores8_gather_kernel(const dsaspp_scores8_desc d, const int tiles_x, const int tiles_y, const unsigned per_line,
+                                                             const int64_t lines) {
     const bool inner = d.gc == 1;
-    for (int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x; idx < total; idx += (int64_t)gridDim.x * 256) {
-        int64_t t = idx;
-        int c, x, y;
-        if (inner) {
-            c = (int)(t % d.n_class); t /= d.n_class;
-            x = (int)(t % d.w); t /= d.w;
-            y = (int)(t % d.h); t /= d.h;
-        } else {
-            x = (int)(t % d.w); t /= d.w;
-            y = (int)(t % d.h); t /= d.h;
-            c = (int)(t % d.n_class); t /= d.n_class;
+    const unsigned i = blockIdx.x * 256 + threadIdx.x;
+    if (i >= per_line) return;
+    const int c = inner ? i % (unsigned)d.n_class : i / (unsigned)d.w, x = inner ? i / (unsigned)d.n_class : i % (unsigned)d.w;
+    const Span sx(x, d.w);
+    for (int64_t line0 = (int64_t)blockIdx.y * GL; line0 < lines; line0 += (int64_t)gridDim.y * GL) {
+        float v[GL][4];
+        auto at = [&](int n, int uy, int ty, int ux, int tx) {
+            return d.ws[((((int64_t)n * tiles_y + ty) * tiles_x + tx) * (PX * PY) + (uy - ty * TCY) * PX + (ux - tx * TCX)) * d.n_class + c];
+        };
+#pragma unroll
+        for (int k = 0; k < GL; ++k) {
+#pragma unroll
+            for (int m = 0; m < 4; ++m) v[k][m] = 0.f;
+            if (line0 + k >= lines) continue;
+            const int n = (int)((line0 + k) / d.h), y = (int)((line0 + k) - (int64_t)n * d.h), uy = y + 1, ux = x + 1;
+            const int ty = uy / TCY, tx = ux / TCX;
+            const bool y0 = ty < tiles_y, y1 = ty > 0 && uy == ty * TCY, x0 = tx < tiles_x, x1 = tx > 0 && ux == tx * TCX;
+            if (y0 && x0) v[k][0] = at(n, uy, ty, ux, tx);
+            if (y0 && x1) v[k][1] = at(n, uy, ty, ux, tx - 1);
+            if (y1 && x0) v[k][2] = at(n, uy, ty - 1, ux, tx);
+            if (y1 && x1) v[k][3] = at(n, uy, ty - 1, ux, tx - 1);
         }
-        const int64_t n = t;
-        int tx[6], ax[6], ty[6], ay[6];
-        const int kx = places<TCX>(x, d.w, tiles_x, tx, ax), ky = places<TCY>(y, d.h, tiles_y, ty, ay);
-        float v = 0.f;
 #pragma unroll
-        for (int j = 0; j < 6; ++j)
-#pragma unroll
-            for (int i = 0; i < 6; ++i)
-                if (j < ky && i < kx) v += d.ws[(((n * tiles_y + ty[j]) * tiles_x + tx[i]) * (PX * PY) + ay[j] * PX + ax[i]) * d.n_class + c];
-        const int64_t o = n * d.gn + y * d.gy + x * d.gx + c * d.gc;
-        if (d.g_dtype == 1) reinterpret_cast<float*>(d.dlogits)[o] = v;
-        else reinterpret_cast<u16*>(d.dlogits)[o] = d.g_dtype == 0 ? Elem<0>::down(v) : Elem<2>::down(v);
+        for (int k = 0; k < GL; ++k) {
+            if (line0 + k >= lines) break;
+            const int n = (int)((line0 + k) / d.h), y = (int)((line0 + k) - (int64_t)n * d.h);
+            float sum = (v[k][0] + v[k][1]) + (v[k][2] + v[k][3]);
+            const Span sy(y, d.h);
+            if (sy.last > sy.first || sx.last > sx.first) {       // border pixels: what fell beyond the border too
+                for (int uy = sy.first; uy <= sy.last; ++uy)
+                    for (int ux = sx.first; ux <= sx.last; ++ux) {
+                        if (uy == y + 1 && ux == x + 1) continue;
+                        for (int ty = first_tile<TCY>(uy); ty <= uy / TCY && ty < tiles_y; ++ty)
+                            for (int tx = first_tile<TCX>(ux); tx <= ux / TCX && tx < tiles_x; ++tx) sum += at(n, uy, ty, ux, tx);
+                    }
+            }
+            const int64_t o = n * d.gn + y * d.gy + x * d.gx + c * d.gc;
+            if (d.g_dtype == 1) reinterpret_cast<float*>(d.dlogits)[o] = sum;
+            else reinterpret_cast<u16*>(d.dlogits)[o] = d.g_dtype == 0 ? Elem<0>::down(sum) : Elem<2>::down(sum);
+        }
     }
 }
 
@@ -427,10 +632,10 @@ extern "C" int dsaspp_scores8_bwd(const dsaspp_scores8_desc* d, dsaspp_stream_t 
 #define F(NC, EX) launch_bwd<NC, EX>(*d, tx, ty, (unsigned)tiles, s)
     BY_CLASSES(F);
 #undef F
-    const int64_t total = (int64_t)d->n_img * d->h * d->w * d->n_class;
-    int64_t nb = (total + 255) / 256;
-    if (nb > (1 << 20)) nb = 1 << 20;
-    hipLaunchKernelGGL(scores8_gather_kernel, dim3((unsigned)nb), dim3(256), 0, s, *d, tx, ty, total);
+    const unsigned per_line = (unsigned)d->w * d->n_class;
+    const int64_t lines = (int64_t)d->n_img * d->h;
+    const int64_t gy = (lines + GL - 1) / GL;
+    hipLaunchKernelGGL(scores8_gather_kernel, dim3((per_line + 255) / 256, (unsigned)(gy < 65535 ? gy : 65535)), dim3(256), 0, s, *d, tx, ty, per_line, lines);
     DS_LAUNCH_CHECK("scores8_bwd");
     return 0;
 }

@@ -2,9 +2,48 @@
 #pragma once
 #include "elem.h"
 #include <float.h>
+#include <type_traits>
 
 constexpr float SR_LOG2E = 1.4426950408889634f, SR_LN2 = 0.6931471805599453f;
 constexpr float SR_FAR = -1000.f;         // stands for any difference whose exponential is 0 (below -150) where the two are multiplied
+
+// Butterfly over neighbouring lanes: the values of the two halves of a group of 2*O lanes whose halves hold one value each.
+// Inside 16 lanes by DPP (quad permutes, then the mirrors of half rows and rows: the halves are uniform by then), across them by the row
+// swaps of gfx950; an LDS permute instead costs about 100 cycles of latency each, and a top-8 over 64 lanes takes 96 in a row.
+template <int O>
+__device__ __forceinline__ void halves(int x, int& a, int& b) {
+    if (O == 1) { a = x; b = __builtin_amdgcn_update_dpp(0, x, 0xB1, 0xF, 0xF, true); }
+    else if (O == 2) { a = x; b = __builtin_amdgcn_update_dpp(0, x, 0x4E, 0xF, 0xF, true); }
+    else if (O == 4) { a = x; b = __builtin_amdgcn_update_dpp(0, x, 0x141, 0xF, 0xF, true); }
+    else if (O == 8) { a = x; b = __builtin_amdgcn_update_dpp(0, x, 0x140, 0xF, 0xF, true); }
+    else if (O == 16) { const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false); a = r[0]; b = r[1]; }
+    else { const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false); a = r[0]; b = r[1]; }
+}
+template <int O>
+__device__ __forceinline__ void halves(float x, float& a, float& b) {
+    int i, j;
+    halves<O>(__float_as_int(x), i, j);
+    a = __int_as_float(i);
+    b = __int_as_float(j);
+}
+// fn<O>() for O = 1, 2, 4 ... LANES/2
+template <int LANES, int O = 1, typename F>
+__device__ __forceinline__ void butterfly(F&& fn) {
+    if constexpr (O < LANES) {
+        fn(std::integral_constant<int, O>());
+        butterfly<LANES, O * 2>(fn);
+    }
+}
+template <int LANES>
+__device__ __forceinline__ float lanes_max(float v) {
+    butterfly<LANES>([&](auto o) { float a, b; halves<decltype(o)::value>(v, a, b); v = fmaxf(a, b); });
+    return v;
+}
+template <int LANES>
+__device__ __forceinline__ unsigned lanes_min(unsigned v) {
+    butterfly<LANES>([&](auto o) { int a, b; halves<decltype(o)::value>((int)v, a, b); v = min((unsigned)a, (unsigned)b); });
+    return v;
+}
 
 // With d = (z - m) log2 e:  s = sum 2^d,  t = sum d 2^d.  The running maximum starts at the lowest finite value, so a row of
 // nothing but -inf keeps s == 0 and any finite logit makes s >= 1.  A NaN or +inf makes s NaN and nothing takes that back.
@@ -30,6 +69,18 @@ struct Soft {
         shift_to(mn);
         s += o.s;
         t += o.t;
+    }
+    // over LANES neighbouring lanes, the same bits in all of them
+    template <int LANES>
+    __device__ __forceinline__ void join_lanes() {
+        butterfly<LANES>([&](auto o) {
+            constexpr int O = decltype(o)::value;
+            Soft b;
+            halves<O>(m, m, b.m);
+            halves<O>(s, s, b.s);
+            halves<O>(t, t, b.t);
+            join(b.m, b.s, b.t);
+        });
     }
     __device__ __forceinline__ bool empty() const { return s == 0.f; }
     __device__ __forceinline__ float entropy(float log_s) const {
@@ -62,20 +113,14 @@ struct Top {
             v[0] = g[0] ? z : v[0];
         }
     }
-    // The K largest of the lists of 2^n neighbouring lanes, in every one of them: K times the best head, whose lane moves up.
+    // The K largest of the lists of LANES neighbouring lanes, in every one of them: K times the best head, whose lane moves up.
     template <int LANES>
     __device__ __forceinline__ void join_lanes() {
         Top<K> r;
 #pragma unroll
         for (int j = 0; j < K; ++j) {
-            float bv = v[0];
-            int bi = i[0];
-#pragma unroll
-            for (int o = 1; o < LANES; o <<= 1) {
-                const float ov = __shfl_xor(bv, o, 64);
-                const int oi = __shfl_xor(bi, o, 64);
-                if (ov > bv || (ov == bv && (unsigned)oi < (unsigned)bi)) { bv = ov; bi = oi; }
-            }
+            const float bv = lanes_max<LANES>(v[0]);
+            const int bi = (int)lanes_min<LANES>(v[0] == bv ? (unsigned)i[0] : 0xffffffffu);       // -1, no class, is the largest
             const bool mine = bi >= 0 && i[0] == bi;
 #pragma unroll
             for (int q = 0; q + 1 < K; ++q) {

@@ -12,12 +12,16 @@ def tiny(dtype):
     return torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps      # spacing below the normal range
 
 
-def scores(z, labels, top_k, ignore_index, terms):
+def scores(z, labels, top_k, ignore_index, terms, R=0.0):
     """z: N x C x ... any float type; everything returned in float64 / int64, with absolute tolerances.  `terms`: additions that
     one running sum of the kernel may hold in a row.
 
     With d = z - m (one rounding, relative U), e = exp(d) is off by at most (2|d| + 2) U, so s = sum e by (terms + 2 + 2 sum p|d|) U, and
-    sum p|d| = H - log s <= H.  t = sum d e likewise, relative to sum |d| e = s (H - log s).  log adds 2 U (1 + log s), log s <= H."""
+    sum p|d| = H - log s <= H.  t = sum d e likewise, relative to sum |d| e = s (H - log s).  log adds 2 U (1 + log s), log s <= H.
+
+    R > 0: the x8 form on logits of magnitude up to R, which takes each exponential from the one of the row above.  Its logarithm is off by
+    delta = 15 R U (the reference's own interpolation included) + 23 U (7 steps of 3 U, the first exponential); d is counted from a
+    reference up to 2 R off the maximum, so that log s and t / s are 2 R larger before they cancel."""
     zd = z.detach().double().cpu()
     c = zd.shape[1]
     bad = (torch.isnan(zd) | torch.isposinf(zd)).any(1)
@@ -33,8 +37,10 @@ def scores(z, labels, top_k, ignore_index, terms):
     h = torch.where(bad, float('nan'), h)
     hh = torch.where(bad, 0.0, h)
     out = dict(p=p, lp=lp, entropy=h, empty=empty, bad=bad)
-    out['entropy_tol'] = U * (2 * terms + 16) * (1 + hh)
-    base = U * ((terms + 8) * (1 + hh) + 4 * hh)
+    delta = 15 * R * U + 23 * U if R else 0.0
+    out['delta'], out['shift'] = delta, 2.0 * R
+    out['entropy_tol'] = U * (2 * terms + 16) * (1 + hh) + 2 * delta * (1 + 2 * hh) + (terms + 8) * U * 2 * R
+    base = U * ((terms + 8) * (1 + hh) + 4 * hh) + 2 * delta + 8 * U * R
     if labels is not None:
         lab = labels.cpu()
         has = (lab != ignore_index) & (lab >= 0) & (lab < c)
@@ -90,7 +96,8 @@ def gradient(r, g_logp, g_entropy, g_top, terms):
     g = torch.where(alive, g, 0.0)
     inner = size.unsqueeze(1) + b.abs().unsqueeze(1) * (lpf.abs() + h.unsqueeze(1))
     tol = U * ((terms + 16 + 4 * lpf.abs()) * p * inner + (terms + 16) * b.abs().unsqueeze(1) * p * (1 + h.unsqueeze(1)) + 4 * delta.abs() + 10 * size.unsqueeze(1) * (delta != 0))
-    tol = torch.where(alive & ~r['bad'].unsqueeze(1), tol, 0.0)
+    more = 2 * r['delta'] * p * inner + b.abs().unsqueeze(1) * p * (2 * r['delta'] + (terms + 8) * U * r['shift'])
+    tol = torch.where(alive & ~r['bad'].unsqueeze(1), tol + more, 0.0)
     return g, tol
 
 

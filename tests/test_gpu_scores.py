@@ -251,7 +251,7 @@ def test_gradient_against_differences():
 def _check8(z, labels, low, top_k, train, entropy=True, ups_mask=None, ignore_index=-100):
     c = z.shape[1]
     full = R.interpolate(z)
-    r = R.scores(full, labels, top_k, ignore_index, c)
+    r = R.scores(full, labels, top_k, ignore_index, c, R=_size(z))
     if train:
         low = low.detach().requires_grad_()
     s = _label_scores(low, None if labels is None else labels.cuda(), top_k=top_k, ignore_index=ignore_index, entropy=entropy, upsample=8)
@@ -287,6 +287,12 @@ def _check8(z, labels, low, top_k, train, entropy=True, ups_mask=None, ignore_in
     lim = R.adjoint(tol) + 64 * R.U * R.adjoint(size)
     assert grad.dtype == low.dtype and grad.shape == low.shape
     R.agree(grad, R.adjoint(want), lim, 'gradient', low.dtype)
+
+
+def _size(low):
+    """Magnitude of the logits where the short form applies (below 1e5), else 0: the other form is the plain one."""
+    big = float(low.detach().float().abs().max())
+    return big if big < 1e5 else 0.0
 
 
 def _make8(shape, dtype, layout, seed, ints=False):
@@ -334,6 +340,32 @@ def test_upsampled_ties_and_lowest_values():
     _check8(z, labels, low, 4, True)
     z[:, 3:] = -1e30                                   # finite masks
     _check8(z, labels, _place(z, 'last'), 3, True)
+
+
+@pytest.mark.parametrize('classes', [5, 19, 30])
+@pytest.mark.parametrize('depth', [100.0, 3000.0, 1e10, 1e19, 3e20])
+def test_upsampled_rows_that_peak_at_different_classes(depth, classes):
+    """Neighbouring pixels hundreds of units (and far more) apart in opposite classes: between them every class is far below either
+    peak."""
+    z, labels, low = _make8((1, classes, 4, 6), torch.float32, 'last', 7)
+    z = (z - depth)
+    z[:, 0, ::2, ::2] += depth
+    z[:, 1, 1::2, ::2] += depth
+    z[:, 2, ::2, 1::2] += depth
+    z[:, 3, 1::2, 1::2] += depth
+    _check8(z, labels, _place(z, 'last'), 3, True)
+    _check8(z, labels, _place(z, 'last'), 0, True)
+
+
+@pytest.mark.parametrize('k', [2, 3, 8])
+def test_upsampled_near_ties(k):
+    """Classes that differ in their last bits alone, in both directions, and both zeros."""
+    g = torch.Generator().manual_seed(k)
+    base = torch.randn(1, 1, 5, 6, generator=g).expand(1, 19, 5, 6)
+    z = base * (1 + torch.randint(-3, 4, (1, 19, 5, 6), generator=g) * 2.0 ** -23)
+    z = torch.where(torch.rand(1, 1, 5, 6, generator=g) < 0.2, torch.randn(1, 19, 5, 6, generator=g).sign() * 0.0, z)
+    labels = torch.randint(0, 19, (1, 40, 48), generator=g)
+    _check8(z, labels, _place(z, 'last'), k, True)
 
 
 def test_upsampled_nan_stays_where_it_is_read():
@@ -450,7 +482,7 @@ def test_network_scores_are_those_of_its_logits():
     s = mod.score(x.cuda(), labels.cuda(), top_k=3)
     low = mod.forward_lowres(x.cuda())
     full = R.interpolate(low)
-    r = R.scores(full, labels, 3, 255, 19)
+    r = R.scores(full, labels, 3, 255, 19, R=_size(low))
     R.agree(s.logp, r['logp'], r['logp_tol'], 'logp')
     R.agree(s.entropy, r['entropy'], r['entropy_tol'], 'entropy')
     assert torch.equal(s.top_class.cpu(), r['top_class'])
@@ -499,7 +531,7 @@ def test_scores_of_a_training_step_agree_with_its_fused_loss():
     mine = -s.logp.sum() / count
     assert abs(float(mine.detach()) - loss) <= 64 * R.U * loss                 # two sums of 1e4 terms of one sign, trees of fewer than 64 roundings
     grad, = torch.autograd.grad(mine, low)
-    r = R.scores(R.interpolate(low), labels, 0, 255, 19)
+    r = R.scores(R.interpolate(low), labels, 0, 255, 19, R=_size(low))
     u = torch.full(labels.shape, -1.0 / count)
     want, tol = R.gradient(r, u, None, None, 19)
     lim = 2 * (R.adjoint(tol) + 64 * R.U * R.adjoint(want.abs() + r['p'] / count))

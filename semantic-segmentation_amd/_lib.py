@@ -185,6 +185,7 @@ def load():
     lib.dsaspp_stem7_wgrad_workspace_floats.argtypes = [ctypes.c_int32]
     lib.dsaspp_stem7_wgrad_workspace_floats.restype = ctypes.c_int64
     lib.dsaspp_grad_ranges_overlap.argtypes = [ctypes.POINTER(clip_desc)]
+    lib.dsaspp_grad_ranges_overlap.restype = ctypes.c_int
     lib.dsaspp_grad_norm_workspace.argtypes = [ctypes.POINTER(clip_desc)]
     lib.dsaspp_grad_norm_workspace.restype = ctypes.c_int64
     lib.dsaspp_adam_step_clipped.argtypes = [ctypes.POINTER(adam_clip_desc), ctypes.POINTER(clip_desc), ctypes.c_void_p]
@@ -234,28 +235,33 @@ def check(rc):
         raise DsasppError(load().dsaspp_last_error().decode('utf-8', 'replace'))
 
 
-class _Here:
-    def __enter__(self):
-        pass
-
-    def __exit__(self, *a):
-        pass
+_binding = None
 
 
-_HERE = _Here()
+def binding():
+    """The torch binding of the class-score and gradient-norm operators (csrc/torch_binding.cpp), tied to the loaded library.  Raises
+    if it is missing."""
+    global _binding
+    if _binding is None:
+        import importlib.machinery
+        import importlib.util
+        import torch  # noqa: F401  (the binding's symbols come from it)
+        path = os.path.join(HERE, '_dsaspp_torch.so')
+        if not os.path.exists(path):
+            raise DsasppError('%s not found -- build it with `python semantic-segmentation_amd/build.py`; there is no fallback' % path)
+        loader = importlib.machinery.ExtensionFileLoader('_dsaspp_torch', path)
+        mod = importlib.util.module_from_spec(importlib.util.spec_from_file_location('_dsaspp_torch', path, loader=loader))
+        loader.exec_module(mod)
+        lib = load()
+        mod.init({n: ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in exported_symbols()})
+        _binding = mod
+    return _binding
 
 
-def on_device(t):
-    """Context in which the device of tensor t is the current one."""
+def raw_stream(t):
+    """hipStream_t of the current stream of tensor t's GPU, as an integer (0 for a tensor that is on none)."""
     import torch
-    index = t.get_device()
-    return _HERE if index == torch.cuda.current_device() else torch.cuda.device(index)
-
-
-def raw_stream(index):
-    """hipStream_t of the current stream of device `index`, as an integer."""
-    import torch
-    return torch._C._cuda_getCurrentRawStream(index)
+    return torch._C._cuda_getCurrentRawStream(t.get_device()) if t.is_cuda else 0
 
 
 def exported_symbols():

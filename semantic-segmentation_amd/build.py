@@ -52,6 +52,50 @@ def library_hash():
     return m.group(1).decode() if m else None
 
 
+# Python binding of the operators called on lists of tensors and through autograd (csrc/torch_binding.cpp): host code, g++ against the
+# installed torch
+BINDING = os.path.join(HERE, '_dsaspp_torch.so')
+BINDING_SOURCE = os.path.join(CSRC, 'torch_binding.cpp')
+BINDING_FLAGS = ['-O2', '-std=c++17', '-fPIC', '-shared', '-Wall']
+
+
+def binding_hash():
+    """Hash of what the binding is compiled from: its source, the public header, the flags and the torch version."""
+    import hashlib
+    from torch.version import __version__ as torch_version
+    h = hashlib.sha256(' '.join(BINDING_FLAGS + [str(torch_version), '%d.%d' % sys.version_info[:2]]).encode())
+    for path in (BINDING_SOURCE, os.path.join(INCLUDE, 'dsaspp.h')):
+        h.update(open(path, 'rb').read())
+    return h.hexdigest()[:16]
+
+
+def built_binding_hash():
+    if not os.path.exists(BINDING):
+        return None
+    import re
+    m = re.search(rb'DSASPP_BIND=([0-9a-f]{16})', open(BINDING, 'rb').read())
+    return m.group(1).decode() if m else None
+
+
+def build_binding(force=False, verbose=False):
+    bh = binding_hash()
+    if not force and built_binding_hash() == bh:
+        return BINDING
+    import sysconfig
+    import torch
+    root = os.path.dirname(torch.__file__)
+    inc = [INCLUDE, os.path.join(root, 'include'), os.path.join(root, 'include', 'torch', 'csrc', 'api', 'include'),
+           sysconfig.get_paths()['include']]
+    cmd = ['g++', *BINDING_FLAGS, '-DDSASPP_BINDING_HASH="%s"' % bh]
+    for d in inc:
+        cmd += ['-isystem' if d != INCLUDE else '-I', d]
+    cmd += [BINDING_SOURCE, '-o', BINDING, '-L' + os.path.join(root, 'lib'), '-ltorch_python', '-ltorch_cpu', '-ltorch', '-lc10']
+    if verbose:
+        print(' '.join(cmd))
+    subprocess.check_call(cmd)
+    return BINDING
+
+
 def build_library(force=False, verbose=False, extra_flags=(), out=None):
     """Build the library.  With extra_flags (diagnostic builds, results possibly wrong on purpose) an explicit output
     path is required: the in-tree product library is only ever written by a build with the product flags."""
@@ -99,3 +143,4 @@ def build_library(force=False, verbose=False, extra_flags=(), out=None):
 
 if __name__ == '__main__':
     print(build_library(force='--force' in sys.argv, verbose=True))
+    print(build_binding(force='--force' in sys.argv, verbose=True))

@@ -22,7 +22,8 @@ import torch.nn as nn
 from . import spec as S
 from .arena import ParamArena
 from .engine import Engine
-from .scores import Scores, _Plan
+from . import _lib
+from .scores import Scores
 
 _LEGACY = re.compile(r'\.(norm|relu|conv)\.(\d)\.')
 
@@ -108,15 +109,14 @@ class _ScoreFn(torch.autograd.Function):
     logits of the engine."""
 
     @staticmethod
-    def forward(ctx, model, x, plan, dropout_masks, generator, *params):
-        eng = model._run_forward(x, dropout_masks=dropout_masks, generator=generator)
-        s, _ = plan.forward(eng.low_logits(), False)
-        ctx.model, ctx.eng, ctx.plan, ctx.pass_id = model, eng, plan, eng.pass_id
+    def forward(ctx, model, x, args, dropout_masks, generator, *params):
+        eng, s = model._scored_pass(x, args, dropout_masks, generator)
+        ctx.model, ctx.eng, ctx.ignore_index, ctx.pass_id = model, eng, args[2], eng.pass_id
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(s.top_class, plan.labels)
-        if s.top_class is not None:
-            ctx.mark_non_differentiable(s.top_class)
-        return tuple(s)
+        ctx.save_for_backward(s[3], args[0])
+        if s[3] is not None:
+            ctx.mark_non_differentiable(s[3])
+        return s
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -126,9 +126,10 @@ class _ScoreFn(torch.autograd.Function):
             raise RuntimeError('DenseASPP.score: another pass has run since this forward pass and its activations are gone; '
                                'call backward once, before the next pass')
         eng.pass_id += 1
-        top_class, _ = ctx.saved_tensors
+        top_class, labels = ctx.saved_tensors
+        low = eng.low_logits()
         dlow = eng.dlogits.view(eng.B, eng.H2, eng.W2, S.CLS_PAD)[..., :model.spec.n_class].permute(0, 3, 1, 2)
-        ctx.plan.backward(eng.low_logits(), None, None, top_class, g_logp, g_entropy, g_top, out=dlow)
+        _lib.binding().upsampled_backward(low, labels, ctx.ignore_index, top_class, g_logp, g_entropy, g_top, dlow, _lib.raw_stream(low))
         # as in _LogitsFn: the arena the .grad views alias keeps its contents
         held = model._gflat.clone()
         model._gflat_zero()
@@ -495,11 +496,18 @@ class DenseASPP(nn.Module):
             raise ValueError('DenseASPP expects an N x 3 x H x W image batch, got %s' % (tuple(x.shape),))
         if x.shape[2] % 8 or x.shape[3] % 8:
             raise ValueError('DenseASPP.score: H and W must be multiples of 8, got %d x %d' % tuple(x.shape[2:]))
-        plan = _Plan((x.shape[0], self.spec.n_class, x.shape[2] // 8, x.shape[3] // 8), x.device, labels, top_k, ignore_index, entropy, 8)
+        args = (labels, int(top_k), int(ignore_index), bool(entropy))
+        # before the pass, which updates running statistics in train() mode
+        _lib.binding().check_scores([x.shape[0], self.spec.n_class, x.shape[2] // 8, x.shape[3] // 8], str(x.device), labels, args[1], args[3], 8)
         if torch.is_grad_enabled() and self.training:
-            return Scores(*_ScoreFn.apply(self, x, plan, dropout_masks, generator, *[p for _, p in self.named_parameters()]))
+            return Scores._make(_ScoreFn.apply(self, x, args, dropout_masks, generator, *[p for _, p in self.named_parameters()]))
+        return Scores._make(self._scored_pass(x, args, dropout_masks, generator)[1])
+
+    def _scored_pass(self, x, args, dropout_masks, generator):
+        labels, top_k, ignore_index, entropy = args
         eng = self._run_forward(x, dropout_masks=dropout_masks, generator=generator)
-        return plan.forward(eng.low_logits(), False)[0]
+        low = eng.low_logits()
+        return eng, _lib.binding().upsampled_forward(low, labels, top_k, ignore_index, entropy, _lib.raw_stream(low))
 
     def train_step(self, x, labels, ignore_index=255, dropout_masks=None, generator=None, zero_grad=True,
                    refresh=True, reducer=None):

@@ -584,7 +584,9 @@ typedef struct dsaspp_scores_desc {
     const float* g_logp; const float* g_entropy; const float* g_top;
     int32_t g_logp_one, g_entropy_one, g_top_one;
     void* dlogits;
+    float* ws; int64_t ws_len; /* forward, few long rows: dsaspp_scores_workspace floats, contents need not be initialised */
 } dsaspp_scores_desc;
+int64_t dsaspp_scores_workspace(const dsaspp_scores_desc* d); /* floats for the forward call, often 0; -1 on a bad descriptor */
 int dsaspp_scores_fwd(const dsaspp_scores_desc* d, dsaspp_stream_t stream);
 int dsaspp_scores_bwd(const dsaspp_scores_desc* d, dsaspp_stream_t stream);
 

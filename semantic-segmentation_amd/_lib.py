@@ -189,6 +189,8 @@ def load():
     lib.dsaspp_grad_norm_workspace.argtypes = [ctypes.POINTER(clip_desc)]
     lib.dsaspp_grad_norm_workspace.restype = ctypes.c_int64
     lib.dsaspp_adam_step_clipped.argtypes = [ctypes.POINTER(adam_clip_desc), ctypes.POINTER(clip_desc), ctypes.c_void_p]
+    lib.dsaspp_scores_workspace.argtypes = [ctypes.POINTER(scores_desc)]
+    lib.dsaspp_scores_workspace.restype = ctypes.c_int64
     lib.dsaspp_scores8_workspace.argtypes = [ctypes.POINTER(scores8_desc)]
     lib.dsaspp_scores8_workspace.restype = ctypes.c_int64
     lib.dsaspp_set_comm_cus.argtypes = [ctypes.c_int32]

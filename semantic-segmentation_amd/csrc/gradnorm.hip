@@ -14,25 +14,34 @@
 
 namespace {
 
-constexpr int MAX_RANGES = 180;           // ranges that travel in the kernel arguments of one launch (3.6 of 4 KB)
 constexpr int CHUNK = 8192;               // elements of one range that a block takes at a time
 constexpr int MAX_BLOCKS = 2048;          // 8 blocks of 4 waves per CU fill the chip; a block takes several chunks in a row
-constexpr int64_t MAX_ELEMS = (int64_t)CHUNK << 29;     // chunks of one launch count in 32 bits
+// The ranges of one launch travel in its kernel arguments (4.0 of 4 KB), ten bytes each: 32 bits of distance from the first range, in
+// elements, 32 bits of length and 16 bits of first chunk.  24 bytes each made three launches of what fits one; a launch costs the host 3 us.
+constexpr int MAX_RANGES = 400;
+constexpr int MAX_CHUNKS = 65535;         // of one launch
+constexpr int64_t MAX_LENGTH = (int64_t)(MAX_CHUNKS / 2) * CHUNK;       // of one range; longer ones are several
+constexpr int64_t MAX_ELEMS = (int64_t)1 << 42;
 
 struct Group {
-    void* p[MAX_RANGES];
-    int64_t n[MAX_RANGES];
-    int32_t first[MAX_RANGES + 1];        // first chunk of range i
+    char* base;
+    int32_t at[MAX_RANGES];               // in elements from base
+    uint32_t n[MAX_RANGES];
+    uint16_t first[MAX_RANGES + 1];       // first chunk of range i
     int32_t n_ranges;
 };
+static_assert(sizeof(Group) <= 4032, "kernel arguments beside it: workspace, counts, threshold, result");
 
+// Last range whose first chunk is <= chunk: every lane compares some, all loads at once.
 __device__ __forceinline__ int find_range(const Group& g, int chunk) {
-    int lo = 0, hi = g.n_ranges - 1;      // last range whose first chunk is <= chunk
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (g.first[mid] <= chunk) lo = mid; else hi = mid - 1;
+    const int lane = threadIdx.x & 63;
+    int r = 0;
+#pragma unroll
+    for (int k = 0; k < MAX_RANGES; k += 64) {
+        const int i = k + lane;
+        r += __popcll(__ballot(i > 0 && i < g.n_ranges && (int)g.first[i < MAX_RANGES ? i : MAX_RANGES] <= chunk));
     }
-    return lo;
+    return r;
 }
 
 // Consecutive chunks of this block: the range is looked up once.  Every block has at least one (the grid has no more blocks).
@@ -73,10 +82,9 @@ __global__ __launch_bounds__(256) void partials_kernel(const Group g, double* ws
     int r = find_range(g, sh.first);
     for (int ch = sh.first; ch < sh.last; ++ch) {
         while (ch >= g.first[r + 1]) ++r;
-        const int64_t off = (int64_t)(ch - g.first[r]) * CHUNK;
-        const int64_t left = g.n[r] - off;
+        const uint32_t off = (uint32_t)(ch - g.first[r]) * CHUNK, left = g.n[r] - off;
         const int n = left < CHUNK ? (int)left : CHUNK;
-        const typename E::T* p = reinterpret_cast<const typename E::T*>(g.p[r]) + off;
+        const typename E::T* p = reinterpret_cast<const typename E::T*>(g.base) + g.at[r] + off;
         constexpr int IT = CHUNK / E::N / 256;                  // loads in flight before the first is used
         int i = threadIdx.x * E::N;
         for (; i + ((IT - 1) * 256 + 1) * E::N <= n; i += IT * 256 * E::N) {
@@ -140,10 +148,9 @@ __global__ __launch_bounds__(256) void scale_kernel(const Group g, const double*
     int r = find_range(g, sh.last - 1);
     for (int ch = sh.last - 1; ch >= sh.first; --ch) {                  // backwards: what the norm read last is still in the cache
         while (ch < g.first[r]) --r;
-        const int64_t off = (int64_t)(ch - g.first[r]) * CHUNK;
-        const int64_t left = g.n[r] - off;
+        const uint32_t off = (uint32_t)(ch - g.first[r]) * CHUNK, left = g.n[r] - off;
         const int n = left < CHUNK ? (int)left : CHUNK;
-        typename E::T* p = reinterpret_cast<typename E::T*>(g.p[r]) + off;
+        typename E::T* p = reinterpret_cast<typename E::T*>(g.base) + g.at[r] + off;
         constexpr int IT = CHUNK / E::N / 512;
         int i = threadIdx.x * E::N;
         for (; i + ((IT - 1) * 256 + 1) * E::N <= n; i += IT * 256 * E::N) {
@@ -226,32 +233,42 @@ int blocks_for(int64_t chunks) { return (int)(chunks < MAX_BLOCKS ? chunks : MAX
 template <typename F>
 void for_each_group(const dsaspp_clip_desc& d, F fn) {
     for (int dt = 0; dt < 3; ++dt) {
+        const int64_t size = dt == 1 ? 4 : 2;
         Group g;
-        int64_t total = 0;
+        int64_t chunks = 0;               // of the ranges in g
         const char* end = nullptr;
         g.n_ranges = 0;
+        g.first[0] = 0;
         auto flush = [&]() {
-            if (g.n_ranges == 0) return;
-            g.first[0] = 0;
-            for (int i = 0; i < g.n_ranges; ++i) g.first[i + 1] = g.first[i] + (int32_t)((g.n[i] + CHUNK - 1) / CHUNK);
-            fn(dt, g);
+            if (g.n_ranges) fn(dt, g);
             g.n_ranges = 0;
-            total = 0;
+            chunks = 0;
             end = nullptr;
         };
         for (int i = 0; i < d.n_ranges; ++i) {
-            const dsaspp_grad_range& r = d.ranges[i];
-            if (r.dtype != dt) continue;
-            if (total > MAX_ELEMS - r.n) flush();
-            if (g.n_ranges > 0 && end == (const char*)r.p) {
-                g.n[g.n_ranges - 1] += r.n;
-            } else {
-                if (g.n_ranges == MAX_RANGES) flush();
-                g.p[g.n_ranges] = r.p;
-                g.n[g.n_ranges++] = r.n;
+            if (d.ranges[i].dtype != dt) continue;
+            char* p = (char*)d.ranges[i].p;
+            for (int64_t left = d.ranges[i].n; left > 0;) {
+                const int64_t n = left < MAX_LENGTH ? left : MAX_LENGTH, more = (n + CHUNK - 1) / CHUNK;
+                const int k = g.n_ranges - 1;
+                if (k >= 0 && end == p && g.n[k] + n <= MAX_LENGTH && chunks + more <= MAX_CHUNKS) {
+                    g.n[k] += (uint32_t)n;
+                    chunks = g.first[k] + ((int64_t)g.n[k] + CHUNK - 1) / CHUNK;
+                    g.first[k + 1] = (uint16_t)chunks;
+                } else {
+                    const int64_t at = k >= 0 ? (p - g.base) / size : 0;
+                    // a distance that is no whole number of elements or needs more than 32 bits starts a launch of its own
+                    if (g.n_ranges == MAX_RANGES || chunks + more > MAX_CHUNKS || (k >= 0 && ((p - g.base) % size != 0 || at != (int32_t)at))) flush();
+                    if (g.n_ranges == 0) g.base = p;
+                    g.at[g.n_ranges] = (int32_t)((p - g.base) / size);
+                    g.n[g.n_ranges] = (uint32_t)n;
+                    chunks += more;
+                    g.first[++g.n_ranges] = (uint16_t)chunks;
+                }
+                p += n * size;
+                end = p;
+                left -= n;
             }
-            total += r.n;
-            end = (const char*)r.p + r.n * (dt == 1 ? 4 : 2);
         }
         flush();
     }
@@ -277,12 +294,38 @@ int64_t n_partials(const dsaspp_clip_desc& d) {
     return n;
 }
 
+int check_used(const dsaspp_clip_desc* d, const char* who, int64_t used) {
+    DS_REQUIRE(used < (1ll << 31), "%s: too many ranges", who);
+    DS_REQUIRE(used == 0 || (d->ws && d->ws_len >= used && ((uintptr_t)d->ws & 7) == 0), "%s: the workspace needs %lld doubles", who, (long long)used);
+    return 0;
+}
+
 int check_ws(const dsaspp_clip_desc* d, const char* who, int64_t* used) {
     if (int rc = check(d, who)) return rc;
     *used = n_partials(*d);
-    DS_REQUIRE(*used < (1ll << 31), "%s: too many ranges", who);
-    DS_REQUIRE(*used == 0 || (d->ws && d->ws_len >= *used && ((uintptr_t)d->ws & 7) == 0), "%s: the workspace needs %lld doubles", who, (long long)*used);
-    return 0;
+    return check_used(d, who, *used);
+}
+
+void launch_partials(const dsaspp_clip_desc& d, hipStream_t s) {
+    double* ws = d.ws;
+    for_each_group(d, [&](int dt, const Group& g) {
+        const int nb = blocks_for(g.first[g.n_ranges]);
+#define PARTIALS(DT)                                                                                                       \
+        if (d.norm_type == 2) hipLaunchKernelGGL((partials_kernel<DT, false>), dim3(nb), dim3(256), 0, s, g, ws);          \
+        else hipLaunchKernelGGL((partials_kernel<DT, true>), dim3(nb), dim3(256), 0, s, g, ws)
+        if (dt == 0) { PARTIALS(0); } else if (dt == 1) { PARTIALS(1); } else { PARTIALS(2); }
+#undef PARTIALS
+        ws += nb;
+    });
+}
+
+void launch_scale(const dsaspp_clip_desc& d, int used, hipStream_t s) {
+    for_each_group(d, [&](int dt, const Group& g) {
+        const int nb = blocks_for(g.first[g.n_ranges]);
+        if (dt == 0) hipLaunchKernelGGL(scale_kernel<0>, dim3(nb), dim3(256), 0, s, g, d.ws, used, d.norm_type, d.max_norm, d.norm);
+        else if (dt == 1) hipLaunchKernelGGL(scale_kernel<1>, dim3(nb), dim3(256), 0, s, g, d.ws, used, d.norm_type, d.max_norm, d.norm);
+        else hipLaunchKernelGGL(scale_kernel<2>, dim3(nb), dim3(256), 0, s, g, d.ws, used, d.norm_type, d.max_norm, d.norm);
+    });
 }
 
 // Norm and scaling of a few gradients in one block: no second launch, which costs as long as the work.
@@ -294,7 +337,7 @@ __global__ __launch_bounds__(1024) void clip_one_kernel(const Group g, int norm_
     __shared__ double lds[16];
     double acc = 0.0;
     for (int r = 0; r < g.n_ranges; ++r) {
-        const typename E::T* p = reinterpret_cast<const typename E::T*>(g.p[r]);
+        const typename E::T* p = reinterpret_cast<const typename E::T*>(g.base) + g.at[r];
         const int n = (int)g.n[r];
         for (int i = threadIdx.x; i < n; i += 1024) {
             const float x = E::up(p[i]);
@@ -316,7 +359,7 @@ __global__ __launch_bounds__(1024) void clip_one_kernel(const Group g, int norm_
     const float coef = clip_coef(total, max_norm);
     if (coef == 1.f) return;
     for (int r = 0; r < g.n_ranges; ++r) {
-        typename E::T* p = reinterpret_cast<typename E::T*>(g.p[r]);
+        typename E::T* p = reinterpret_cast<typename E::T*>(g.base) + g.at[r];
         const int n = (int)g.n[r];
         for (int i = threadIdx.x; i < n; i += 1024) p[i] = E::down(E::up(p[i]) * coef);
     }
@@ -337,7 +380,7 @@ extern "C" int dsaspp_grad_ranges_overlap(const dsaspp_clip_desc* d) {
         const uintptr_t p = (uintptr_t)d->ranges[i].p;
         v.emplace_back(p, p + (uintptr_t)d->ranges[i].n * (d->ranges[i].dtype == 1 ? 4 : 2));
     }
-    std::sort(v.begin(), v.end());
+    if (!std::is_sorted(v.begin(), v.end())) std::sort(v.begin(), v.end());
     for (size_t i = 1; i < v.size(); ++i)
         if (v[i].first < v[i - 1].second) return 1;
     return 0;
@@ -351,17 +394,7 @@ extern "C" int64_t dsaspp_grad_norm_workspace(const dsaspp_clip_desc* d) {
 extern "C" int dsaspp_grad_norm_partials(const dsaspp_clip_desc* d, dsaspp_stream_t stream) {
     int64_t used = 0;
     if (int rc = check_ws(d, "grad_norm_partials", &used)) return rc;
-    double* ws = d->ws;
-    hipStream_t s = (hipStream_t)stream;
-    for_each_group(*d, [&](int dt, const Group& g) {
-        const int nb = blocks_for(g.first[g.n_ranges]);
-#define PARTIALS(DT)                                                                                                       \
-        if (d->norm_type == 2) hipLaunchKernelGGL((partials_kernel<DT, false>), dim3(nb), dim3(256), 0, s, g, ws);         \
-        else hipLaunchKernelGGL((partials_kernel<DT, true>), dim3(nb), dim3(256), 0, s, g, ws)
-        if (dt == 0) { PARTIALS(0); } else if (dt == 1) { PARTIALS(1); } else { PARTIALS(2); }
-#undef PARTIALS
-        ws += nb;
-    });
+    launch_partials(*d, (hipStream_t)stream);
     DS_LAUNCH_CHECK("grad_norm_partials");
     return 0;
 }
@@ -382,37 +415,34 @@ extern "C" int dsaspp_clip_scale(const dsaspp_clip_desc* d, dsaspp_stream_t stre
     DS_REQUIRE(d->scale == 1.f, "clip_scale: scale must be 1");
     DS_REQUIRE(d->max_norm >= 0.f, "clip_scale: max_norm must be >= 0");
     if (d->n_ranges == 0) return dsaspp_grad_norm_finish(d, stream);
-    hipStream_t s = (hipStream_t)stream;
-    for_each_group(*d, [&](int dt, const Group& g) {
-        const int nb = blocks_for(g.first[g.n_ranges]);
-        if (dt == 0) hipLaunchKernelGGL(scale_kernel<0>, dim3(nb), dim3(256), 0, s, g, d->ws, (int)used, d->norm_type, d->max_norm, d->norm);
-        else if (dt == 1) hipLaunchKernelGGL(scale_kernel<1>, dim3(nb), dim3(256), 0, s, g, d->ws, (int)used, d->norm_type, d->max_norm, d->norm);
-        else hipLaunchKernelGGL(scale_kernel<2>, dim3(nb), dim3(256), 0, s, g, d->ws, (int)used, d->norm_type, d->max_norm, d->norm);
-    });
+    launch_scale(*d, (int)used, (hipStream_t)stream);
     DS_LAUNCH_CHECK("clip_scale");
     return 0;
 }
 
 extern "C" int dsaspp_clip_grads(const dsaspp_clip_desc* d, dsaspp_stream_t stream) {
-    int64_t used = 0;
-    if (int rc = check_ws(d, "clip_grads", &used)) return rc;
+    if (int rc = check(d, "clip_grads")) return rc;
     DS_REQUIRE(d->norm && d->scale == 1.f && d->max_norm >= 0.f, "clip_grads: null output, scale other than 1 or negative max_norm");
-    int64_t total = 0;
+    int64_t total = 0, used = 0;
     int groups = 0;
     for_each_group(*d, [&](int, const Group& g) {
         ++groups;
-        for (int i = 0; i < g.n_ranges; ++i) total += g.n[i] < ONE_BLOCK ? g.n[i] : ONE_BLOCK + 1;
+        used += blocks_for(g.first[g.n_ranges]);
+        for (int i = 0; i < g.n_ranges; ++i) total += g.n[i];
     });
-    if (groups != 1 || total > ONE_BLOCK) {
-        if (int rc = dsaspp_grad_norm_partials(d, stream)) return rc;
-        return dsaspp_clip_scale(d, stream);
-    }
+    if (int rc = check_used(d, "clip_grads", used)) return rc;
     hipStream_t s = (hipStream_t)stream;
-    for_each_group(*d, [&](int dt, const Group& g) {
-        if (dt == 0) hipLaunchKernelGGL(clip_one_kernel<0>, dim3(1), dim3(1024), 0, s, g, d->norm_type, d->max_norm, d->norm);
-        else if (dt == 1) hipLaunchKernelGGL(clip_one_kernel<1>, dim3(1), dim3(1024), 0, s, g, d->norm_type, d->max_norm, d->norm);
-        else hipLaunchKernelGGL(clip_one_kernel<2>, dim3(1), dim3(1024), 0, s, g, d->norm_type, d->max_norm, d->norm);
-    });
+    if (groups == 0) return dsaspp_grad_norm_finish(d, stream);
+    if (groups == 1 && total <= ONE_BLOCK) {
+        for_each_group(*d, [&](int dt, const Group& g) {
+            if (dt == 0) hipLaunchKernelGGL(clip_one_kernel<0>, dim3(1), dim3(1024), 0, s, g, d->norm_type, d->max_norm, d->norm);
+            else if (dt == 1) hipLaunchKernelGGL(clip_one_kernel<1>, dim3(1), dim3(1024), 0, s, g, d->norm_type, d->max_norm, d->norm);
+            else hipLaunchKernelGGL(clip_one_kernel<2>, dim3(1), dim3(1024), 0, s, g, d->norm_type, d->max_norm, d->norm);
+        });
+    } else {
+        launch_partials(*d, s);
+        launch_scale(*d, (int)used, s);
+    }
     DS_LAUNCH_CHECK("clip_grads");
     return 0;
 }

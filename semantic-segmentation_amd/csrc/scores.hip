@@ -8,7 +8,6 @@
 // contiguous: a group of lanes shares a row and reads 16 bytes per lane) and "planes" (class stride other than 1, NCHW: a lane owns
 // P neighbouring pixels and walks the classes).
 #include "softrow.h"
-#include <stdlib.h>
 
 namespace {
 
@@ -135,6 +134,22 @@ __device__ __forceinline__ int load_classes(const typename Elem<DT>::T* z, int c
     return 0;
 }
 
+template <int K>
+__device__ __forceinline__ void store_outputs(const Args& a, int64_t row, const Row& r, int label, float zl, const Soft& s, const Top<K>& top) {
+    const dsaspp_scores_desc& d = a.d;
+    const float log_s = logf(s.s);
+    if (d.logp) d.logp[row] = label_log_p(label, zl, s, log_s);
+    if (d.entropy) d.entropy[row] = s.entropy(log_s);
+    if (d.stats) store_stats(d.stats, row, s, log_s);
+#pragma unroll
+    for (int j = 0; j < K; ++j)
+        if (j < d.top_k) {
+            const int64_t o = (r.i0 * d.top_k + j) * a.plane + r.rem;
+            d.top_logp[o] = top_log_p(top.v[j], top.i[j], s, log_s);
+            d.top_class[o] = top_index(top.i[j], s);
+        }
+}
+
 template <int DT, int K, int TPR>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rows_fwd_kernel(const Args a) {
     typedef Elem<DT> E;
@@ -191,20 +206,91 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rows_fwd_kernel(const A
             s.template join_lanes<WAVES>();
             top.template join_lanes<WAVES>();
         }
-        const float log_s = logf(s.s);
-        if (lane == 0) {
-            if (d.logp) d.logp[row] = label_log_p(label, zl, s, log_s);
-            if (d.entropy) d.entropy[row] = s.entropy(log_s);
-            if (d.stats) store_stats(d.stats, row, s, log_s);
+        if (lane == 0) store_outputs(a, row, r, label, zl, s, top);
+    }
+}
+
+// Few long rows: gridDim.x blocks share a row, each leaving its running values and its K largest; then a wave per row joins them.
+// One block of 1024 lanes takes 13.7 us for a row of 21841 bf16 classes, half of it the vector instructions of a single CU.
+constexpr int MAX_SPLIT = 64;             // partials of a row, one per lane of the wave that joins them
+constexpr int PART = 3 + 2 * DSASPP_SCORES_MAX_TOP;
+
+template <int DT, int K>
+__global__ __launch_bounds__(256) void rows_part_kernel(const Args a, const int span) {
+    typedef Elem<DT> E;
+    __shared__ float ls[4][3];
+    __shared__ float lv[4][K > 0 ? K : 1];
+    __shared__ int li[4][K > 0 ? K : 1];
+    const dsaspp_scores_desc& d = a.d;
+    const int64_t row = blockIdx.y;
+    const Row r = row_of(a, row);
+    const typename E::T* z = reinterpret_cast<const typename E::T*>(d.logits) + r.off;
+    const int c0 = blockIdx.x * span, V = min(d.n_class, c0 + span);        // span is a multiple of 256 N: the last block alone is shorter
+    Soft s;
+    Top<K> top;
+    s.clear();
+    top.clear();
+    for (int c = c0 + threadIdx.x * E::N; c < V; c += 256 * E::N) {
+        float f[E::N];
+        const int base = load_classes<DT>(z, c, V, f);
+        float mx = f[0];
 #pragma unroll
-            for (int j = 0; j < K; ++j)
-                if (j < d.top_k) {
-                    const int64_t o = (r.i0 * d.top_k + j) * a.plane + r.rem;
-                    d.top_logp[o] = top_log_p(top.v[j], top.i[j], s, log_s);
-                    d.top_class[o] = top_index(top.i[j], s);
-                }
+        for (int k = 1; k < E::N; ++k) mx = fmaxf(mx, f[k]);
+        if (mx > s.m) s.shift_to(mx);
+#pragma unroll
+        for (int k = 0; k < E::N; ++k) {
+            s.add(f[k]);
+            top.offer(f[k], base + k);
         }
     }
+    s.template join_lanes<64>();
+    top.template join_lanes<64>();
+    const int wave = threadIdx.x >> 6, wl = threadIdx.x & 63;
+    if (wl == 0) {
+        ls[wave][0] = s.m; ls[wave][1] = s.s; ls[wave][2] = s.t;
+#pragma unroll
+        for (int j = 0; j < K; ++j) { lv[wave][j] = top.v[j]; li[wave][j] = top.i[j]; }
+    }
+    __syncthreads();
+    if (wave != 0) return;
+    s.clear();
+    top.clear();
+    if (wl < 4) {
+        s = Soft{ls[wl][0], ls[wl][1], ls[wl][2]};
+#pragma unroll
+        for (int j = 0; j < K; ++j) { top.v[j] = lv[wl][j]; top.i[j] = li[wl][j]; }
+    }
+    s.template join_lanes<4>();
+    top.template join_lanes<4>();
+    if (wl == 0) {
+        float* o = d.ws + (row * gridDim.x + blockIdx.x) * PART;
+        o[0] = s.m; o[1] = s.s; o[2] = s.t;
+#pragma unroll
+        for (int j = 0; j < K; ++j) { o[3 + 2 * j] = top.v[j]; o[4 + 2 * j] = __int_as_float(top.i[j]); }
+    }
+}
+
+template <int DT, int K>
+__global__ __launch_bounds__(64) void rows_join_kernel(const Args a, const int parts) {
+    typedef Elem<DT> E;
+    const dsaspp_scores_desc& d = a.d;
+    const int64_t row = blockIdx.x;
+    const Row r = row_of(a, row);
+    const int label = label_of(d, row);
+    const float zl = label >= 0 ? E::up(reinterpret_cast<const typename E::T*>(d.logits)[r.off + label]) : 0.f;
+    Soft s;
+    Top<K> top;
+    s.clear();
+    top.clear();
+    if ((int)threadIdx.x < parts) {
+        const float* o = d.ws + (row * parts + threadIdx.x) * PART;
+        s = Soft{o[0], o[1], o[2]};
+#pragma unroll
+        for (int j = 0; j < K; ++j) { top.v[j] = o[3 + 2 * j]; top.i[j] = __float_as_int(o[4 + 2 * j]); }
+    }
+    s.template join_lanes<64>();
+    top.template join_lanes<64>();
+    if (threadIdx.x == 0) store_outputs(a, row, r, label, zl, s, top);
 }
 
 // what the gradient of one row needs besides its logits
@@ -513,14 +599,34 @@ void launch_rows_tpr(const Args& a, hipStream_t s) {
     else hipLaunchKernelGGL((rows_fwd_kernel<DT, K, TPR>), grid, block, 0, s, a);
 }
 
+// Blocks that share a row in the forward pass (1: none do).  Fewer than 128 rows leave half the CUs without a block; a block
+// of a shared row keeps at least one vector per lane.
+int row_parts(const dsaspp_scores_desc& d, int64_t rows) {
+    const int n = d.dtype == 1 ? 4 : 8;
+    if (d.sc != 1 || rows >= 128 || d.n_class < 4 * 256 * n) return 1;
+    const int64_t most = d.n_class / (256 * n), want = 512 / rows;
+    return (int)(most < want ? (most < MAX_SPLIT ? most : MAX_SPLIT) : (want < MAX_SPLIT ? want : MAX_SPLIT));
+}
+int part_span(const dsaspp_scores_desc& d, int parts) {        // classes of a part: whole rounds of the block, so that parts cover the row
+    const int unit = 256 * (d.dtype == 1 ? 4 : 8), per = (d.n_class + parts - 1) / parts;
+    return (per + unit - 1) / unit * unit;
+}
+
+// Lanes per row: 4 hold the lane butterflies and the ends of rows cheap (150 classes: 32 us with 4, 57 with 16, 183 with 64 for 223729 rows);
+// more only as long as the rows are too few to fill the chip, and every lane keeps a vector (1203 classes, 8191 rows: 41 us with 4,
+// 14 with 16, 12 with 64, 20 with 256).
 template <int DT, int K, bool BWD>
 void launch_rows(const Args& a, hipStream_t s) {
-    static const char* e = getenv("TPR");
-    static const int tpr_env = e ? atoi(e) : 0;
     const int64_t vecs = (a.d.n_class + Elem<DT>::N - 1) / Elem<DT>::N;
+    const int parts = BWD ? 1 : row_parts(a.d, a.rows);
+    if (parts > 1) {
+        const int span = part_span(a.d, parts), used = (a.d.n_class + span - 1) / span;
+        hipLaunchKernelGGL((rows_part_kernel<DT, K>), dim3(used, (unsigned)a.rows), dim3(256), 0, s, a, span);
+        hipLaunchKernelGGL((rows_join_kernel<DT, K>), dim3((unsigned)a.rows), dim3(64), 0, s, a, used);
+        return;
+    }
     int tpr = 4;
     while (tpr < 1024 && tpr * 4 <= vecs && a.rows * tpr < 256 * 1024) tpr *= 4;
-    if (tpr_env) tpr = tpr_env;
     if (tpr == 4) launch_rows_tpr<DT, K, 4, BWD>(a, s);
     else if (tpr == 16) launch_rows_tpr<DT, K, 16, BWD>(a, s);
     else if (tpr == 64) launch_rows_tpr<DT, K, 64, BWD>(a, s);
@@ -541,12 +647,22 @@ void launch_k(const Args& a, int k, hipStream_t s) {
 
 }  // namespace
 
+extern "C" int64_t dsaspp_scores_workspace(const dsaspp_scores_desc* d) {
+    Args a;
+    if (check(d, "scores_workspace", &a)) return -1;
+    const int parts = row_parts(*d, a.rows);
+    return parts > 1 ? a.rows * parts * PART : 0;
+}
+
 extern "C" int dsaspp_scores_fwd(const dsaspp_scores_desc* d, dsaspp_stream_t stream) {
     Args a;
     if (int rc = check(d, "scores_fwd", &a)) return rc;
     DS_REQUIRE(!d->logp || d->labels, "scores_fwd: logp needs labels");
     DS_REQUIRE((d->top_k > 0) == (d->top_logp != nullptr) && (d->top_k > 0) == (d->top_class != nullptr), "scores_fwd: top_logp and top_class go with top_k > 0");
     DS_REQUIRE(d->logp || d->entropy || d->stats || d->top_k, "scores_fwd: nothing to compute");
+    const int parts = row_parts(*d, a.rows);
+    DS_REQUIRE(parts == 1 || (d->ws && ((uintptr_t)d->ws & 3) == 0 && d->ws_len >= a.rows * parts * PART), "scores_fwd: the workspace needs %lld floats",
+               (long long)(a.rows * parts * PART));
     hipStream_t s = (hipStream_t)stream;
     if (d->dtype == 0) launch_k<0, false>(a, d->top_k, s);
     else if (d->dtype == 1) launch_k<1, false>(a, d->top_k, s);

@@ -42,6 +42,7 @@ constexpr int64_t MAX_CLASSES_UPSAMPLED = 32;
 struct Api {
     int (*scores_fwd)(const dsaspp_scores_desc*, dsaspp_stream_t);
     int (*scores_bwd)(const dsaspp_scores_desc*, dsaspp_stream_t);
+    int64_t (*scores_workspace)(const dsaspp_scores_desc*);
     int64_t (*scores8_workspace)(const dsaspp_scores8_desc*);
     int (*scores8_fwd)(const dsaspp_scores8_desc*, dsaspp_stream_t);
     int (*scores8_bwd)(const dsaspp_scores8_desc*, dsaspp_stream_t);
@@ -210,6 +211,12 @@ Out scores_forward(const Plan& p, Tensor logits, bool need_stats) {
         fill_common(d, p, logits);
         outputs(d);
         d.stats = ptr<float>(o.stats);
+        const int64_t need = api.scores_workspace(&d);
+        if (need < 0) call(1);
+        Tensor ws;
+        if (need) ws = at::empty({need}, f32);
+        d.ws = ptr<float>(ws);
+        d.ws_len = need;
         call(api.scores_fwd(&d, handle(p.stream)));
     }
     return o;
@@ -539,6 +546,7 @@ void init(const py::dict& f) {
     auto take = [&](const char* name, auto& fn) { fn = reinterpret_cast<std::decay_t<decltype(fn)>>(f[name].cast<int64_t>()); };
     take("dsaspp_scores_fwd", api.scores_fwd);
     take("dsaspp_scores_bwd", api.scores_bwd);
+    take("dsaspp_scores_workspace", api.scores_workspace);
     take("dsaspp_scores8_workspace", api.scores8_workspace);
     take("dsaspp_scores8_fwd", api.scores8_fwd);
     take("dsaspp_scores8_bwd", api.scores8_bwd);

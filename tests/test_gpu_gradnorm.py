@@ -67,10 +67,23 @@ def test_one_tensor(n, dtype):
     _check_clip([t], 0.5)
 
 
-@pytest.mark.parametrize('count', [179, 180, 181, 700])
+@pytest.mark.parametrize('count', [179, 399, 400, 401, 1300])
 def test_many_tensors(count):
     ts = _tensors([(i * 37) % 501 + 1 for i in range(count)], (F32, F32, B16), count)
     _check_clip(ts, 1.0)
+
+
+def test_ranges_longer_than_one_entry_and_launches_longer_than_their_chunks():
+    """3e8 elements: longer than one range of a launch, followed by enough to pass the 65535 chunks of one launch; an odd start between."""
+    buf = torch.ones(300_000_007, dtype=B16, device='cuda')
+    more = torch.ones(280_000_001, dtype=B16, device='cuda')
+    ts = [buf[1:], more, torch.full((5,), 2.0, device='cuda')]
+    want = math.sqrt(300_000_006 + 280_000_001 + 20)
+    _near(_optim().grad_norm(ts), want)
+    _near(_optim().clip_grads_(ts, 0.5 * want), want)
+    half = torch.tensor(0.5 * want / (want + 1e-6)).to(B16)
+    assert bool((ts[0] == half.cuda()).all()) and bool((ts[1] == half.cuda()).all())
+    assert float(buf[0]) == 1.0 and abs(float(ts[2][4]) - 1.0) < 1e-5
 
 
 def test_more_blocks_than_one_launch_keeps():

@@ -123,7 +123,7 @@ def test_rows_of_classes(classes, dtype):
         _check(z, labels, logits, k, True)
 
 
-@pytest.mark.parametrize('rows,classes', [(1, 5003), (3, 8193), (2, 21841), (1030, 8195)])
+@pytest.mark.parametrize('rows,classes', [(1, 5003), (3, 8193), (2, 21841), (1030, 8195), (1, 4096), (1, 100001), (127, 16385), (128, 16385), (20, 4099)])
 @pytest.mark.parametrize('dtype', ['fp32', 'bf16'])
 def test_long_rows(rows, classes, dtype):
     z, labels, logits = _make((rows, classes), DT[dtype], 'last_odd', classes)
@@ -164,7 +164,7 @@ def test_large_planes_in_other_layouts(layout):
 
 @pytest.mark.parametrize('mask', ['random', 'rows', 'lowest', 'nan'])
 @pytest.mark.parametrize('dtype', list(DT))
-@pytest.mark.parametrize('shape', [(64, 5), (40, 19), (9, 150), (5, 3001), (2, 7, 9, 5), (1, 3, 530000)])
+@pytest.mark.parametrize('shape', [(64, 5), (40, 19), (9, 150), (5, 3001), (5, 20001), (2, 7, 9, 5), (1, 3, 530000)])
 def test_masks_infinities_and_nan(shape, dtype, mask):
     z, labels, logits = _make(shape, DT[dtype], 'dense', 11, mask=mask)
     _check(z, labels, logits, min(3, shape[1]), True)
@@ -172,7 +172,7 @@ def test_masks_infinities_and_nan(shape, dtype, mask):
     _check(z, labels, logits, 0, True, g_kind='logp')
 
 
-@pytest.mark.parametrize('shape', [(50, 8), (50, 40), (7, 300), (2, 5000), (2, 19, 7, 9), (1, 20, 530000)])
+@pytest.mark.parametrize('shape', [(50, 8), (50, 40), (7, 300), (2, 5000), (3, 30001), (2, 19, 7, 9), (1, 20, 530000)])
 @pytest.mark.parametrize('k', [1, 2, 3, 8])
 def test_ties_go_to_the_lowest_class(shape, k):
     z, labels, logits = _make(shape, torch.bfloat16, 'dense', k, ints=True)

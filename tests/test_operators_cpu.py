@@ -44,6 +44,18 @@ def test_scores_backward_descriptor(bad, message):
     assert message in _err()
 
 
+def test_scores_workspace_for_few_long_rows():
+    lib = _lib.load()
+    assert lib.dsaspp_scores_workspace(ctypes.byref(_scores())) == 0
+    long = dict(n_class=50000, d0=2, d2=1, s0=50000, sc=1)
+    need = lib.dsaspp_scores_workspace(ctypes.byref(_scores(**long)))
+    assert need > 0 and need % 2 == 0
+    assert lib.dsaspp_scores_workspace(ctypes.byref(_scores(**dict(long, d0=1000)))) == 0
+    assert lib.dsaspp_scores_fwd(ctypes.byref(_scores(**long, ws=GOOD, ws_len=need - 1)), None) != 0
+    assert 'workspace' in _err()
+    assert lib.dsaspp_scores_workspace(ctypes.byref(_scores(dtype=9))) == -1
+
+
 def _scores8(**k):
     d = _lib.scores8_desc()
     f = dict(n_img=1, h=4, w=5, n_class=19, dtype=1, g_dtype=1, sn=380, sy=95, sx=19, sc=1, logits=GOOD, labels=GOOD, ignore_index=255, logp=GOOD)

@@ -11,6 +11,8 @@
 
 namespace {
 
+constexpr int PU = 4;                     // classes a lane has in flight
+
 struct Args {
     dsaspp_scores_desc d;
     int64_t rows, plane;                  // d0*d1*d2, d1*d2
@@ -54,13 +56,16 @@ __device__ __forceinline__ void store_stats(float* stats, int64_t row, const Sof
 }
 
 typedef int64_t i64x2u __attribute__((ext_vector_type(2), aligned(8)));
-// P neighbouring values of a row tensor; np < P only at the end of a row of pixels
+// P neighbouring values of a row tensor (P = 1 or 4), 16 bytes at a time; np < P only at the end of a row of pixels
 template <int P>
 __device__ __forceinline__ void load_row(const float* p, int np, float (&f)[P]) {
-    if (P == 4 && np == P) {
-        const f32x4u v = *reinterpret_cast<const f32x4u*>(p);
+    if (P > 1 && np == P) {
 #pragma unroll
-        for (int k = 0; k < P; ++k) f[k] = v[k & 3];
+        for (int h = 0; h + 3 < P; h += 4) {
+            const f32x4u v = *reinterpret_cast<const f32x4u*>(p + h);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) f[h + k] = v[k];
+        }
     } else {
 #pragma unroll
         for (int k = 0; k < P; ++k) f[k] = k < np ? p[k] : 0.f;
@@ -68,10 +73,13 @@ __device__ __forceinline__ void load_row(const float* p, int np, float (&f)[P]) 
 }
 template <int P>
 __device__ __forceinline__ void load_row(const int64_t* p, int np, int64_t (&f)[P]) {
-    if (P == 4 && np == P) {
-        const i64x2u v = *reinterpret_cast<const i64x2u*>(p), w = *reinterpret_cast<const i64x2u*>(p + 2);
+    if (P > 1 && np == P) {
 #pragma unroll
-        for (int k = 0; k < P; ++k) f[k] = k < 2 ? v[k & 1] : w[k & 1];
+        for (int h = 0; h + 1 < P; h += 2) {
+            const i64x2u v = *reinterpret_cast<const i64x2u*>(p + h);
+            f[h] = v[0];
+            f[h + 1] = v[1];
+        }
     } else {
 #pragma unroll
         for (int k = 0; k < P; ++k) f[k] = k < np ? p[k] : 0;
@@ -79,11 +87,12 @@ __device__ __forceinline__ void load_row(const int64_t* p, int np, int64_t (&f)[
 }
 template <int P>
 __device__ __forceinline__ void store_row(float* p, int np, const float (&f)[P]) {
-    if (P == 4 && np == P) {
-        f32x4u v;
+    if (P > 1 && np == P) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = f[k < P ? k : 0];
-        *reinterpret_cast<f32x4u*>(p) = v;
+        for (int h = 0; h + 3 < P; h += 4) {
+            const f32x4u v = {f[h], f[h + 1], f[h + 2], f[h + 3]};
+            *reinterpret_cast<f32x4u*>(p + h) = v;
+        }
     } else {
 #pragma unroll
         for (int k = 0; k < P; ++k)
@@ -92,11 +101,12 @@ __device__ __forceinline__ void store_row(float* p, int np, const float (&f)[P])
 }
 template <int P>
 __device__ __forceinline__ void store_row(int64_t* p, int np, const int64_t (&f)[P]) {
-    if (P == 4 && np == P) {
-        i64x2u v, w;
-        v[0] = f[0]; v[1] = f[1 % P]; w[0] = f[2 % P]; w[1] = f[3 % P];
-        *reinterpret_cast<i64x2u*>(p) = v;
-        *reinterpret_cast<i64x2u*>(p + 2) = w;
+    if (P > 1 && np == P) {
+#pragma unroll
+        for (int h = 0; h + 1 < P; h += 2) {
+            const i64x2u v = {f[h], f[h + 1]};
+            *reinterpret_cast<i64x2u*>(p + h) = v;
+        }
     } else {
 #pragma unroll
         for (int k = 0; k < P; ++k)
@@ -338,12 +348,13 @@ __device__ __forceinline__ void load_up(const dsaspp_scores_desc& d, int64_t pla
     int label[P];
     float st[2 * P], h[P], ga[P], gb[P];
     load_labels<P>(d, row, np, label);
-    if (P == 4 && np == P) {
-        float lo[4], hi[4];
-        load_row<4>(d.stats + 2 * row, 4, lo);
-        load_row<4>(d.stats + 2 * row + 4, 4, hi);
+    if (P > 1 && np == P) {
 #pragma unroll
-        for (int k = 0; k < 2 * P; ++k) st[k] = k < 4 ? lo[k & 3] : hi[k & 3];
+        for (int h = 0; h + 3 < 2 * P; h += 4) {
+            const f32x4u v = *reinterpret_cast<const f32x4u*>(d.stats + 2 * row + h);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) st[h + k] = v[k];
+        }
     } else {
 #pragma unroll
         for (int k = 0; k < 2 * P; ++k) st[k] = k < 2 * np ? d.stats[2 * row + k] : 0.f;
@@ -419,6 +430,106 @@ __global__ __launch_bounds__(256) void rows_bwd_kernel(const Args a) {
     }
 }
 
+// ---------------------------------------------------------------- rows of few classes: a lane per row, by way of LDS
+// A block's 256 rows are one piece of memory.  It is copied to LDS in 16-byte pieces, every lane takes its row from there (and leaves its
+// gradient there), and no lanes have to be joined.  A row of a multiple of 8 classes gets 16 bytes of padding: its 64 lanes would meet in
+// few LDS banks, and no 16-byte piece crosses its end.
+constexpr int TILE_ROWS = 256, TILE_ROW_BYTES = 128;      // rows of up to 128 bytes: 36 KB of LDS, 4 blocks per CU
+
+template <int DT, bool OUT>
+__device__ __forceinline__ void copy_tile(char* tile, typename Elem<DT>::T* g, int total, int V, int stride) {
+    typedef Elem<DT> E;
+    constexpr int U = 4;
+    const int nv = total / E::N, per_row = V / E::N;
+    const bool padded = stride != V * (int)sizeof(typename E::T);
+    auto place = [&](int i) {
+        const int row = padded ? i / per_row : 0;
+        return reinterpret_cast<typename E::V*>(tile + (padded ? row * stride + (i - row * per_row) * 16 : i * 16));
+    };
+    for (int i0 = threadIdx.x; i0 < nv; i0 += U * 256) {
+        typename E::V v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (i0 + u * 256 < nv) v[u] = OUT ? *place(i0 + u * 256) : *reinterpret_cast<const typename E::V*>(g + (i0 + u * 256) * E::N);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (i0 + u * 256 < nv) {
+                if (OUT) *reinterpret_cast<typename E::V*>(g + (i0 + u * 256) * E::N) = v[u];
+                else *place(i0 + u * 256) = v[u];
+            }
+    }
+    const int i = nv * E::N + (int)threadIdx.x;       // only without padding: a padded tile is whole pieces
+    if (i < total) {
+        if (OUT) g[i] = reinterpret_cast<const typename E::T*>(tile)[i];
+        else reinterpret_cast<typename E::T*>(tile)[i] = g[i];
+    }
+}
+
+template <int DT, int K>
+__global__ __launch_bounds__(256) void tile_fwd_kernel(const Args a, const int stride) {
+    typedef Elem<DT> E;
+    extern __shared__ __attribute__((aligned(16))) char tile[];
+    const dsaspp_scores_desc& d = a.d;
+    const int V = d.n_class;
+    const int64_t row0 = (int64_t)blockIdx.x * TILE_ROWS, row = row0 + threadIdx.x;
+    const int n = a.rows - row0 < TILE_ROWS ? (int)(a.rows - row0) : TILE_ROWS;
+    const int label = (int)threadIdx.x < n ? label_of(d, row) : -1;
+    copy_tile<DT, false>(tile, const_cast<typename E::T*>(reinterpret_cast<const typename E::T*>(d.logits)) + row0 * V, n * V, V, stride);
+    __syncthreads();
+    if ((int)threadIdx.x >= n) return;
+    const typename E::T* z = reinterpret_cast<const typename E::T*>(tile + threadIdx.x * stride);
+    Soft s;
+    Top<K> top;
+    s.clear();
+    top.clear();
+    int c = 0;
+    for (; c + PU <= V; c += PU) {
+        float f[PU];
+#pragma unroll
+        for (int u = 0; u < PU; ++u) f[u] = E::up(z[c + u]);
+        float mx = f[0];
+#pragma unroll
+        for (int u = 1; u < PU; ++u) mx = fmaxf(mx, f[u]);
+        if (mx > s.m) s.shift_to(mx);
+#pragma unroll
+        for (int u = 0; u < PU; ++u) {
+            s.add(f[u]);
+            top.offer(f[u], c + u);
+        }
+    }
+    for (; c < V; ++c) {
+        const float f = E::up(z[c]);
+        if (f > s.m) s.shift_to(f);
+        s.add(f);
+        top.offer(f, c);
+    }
+    store_outputs(a, row, row_of(a, row), label, label >= 0 ? E::up(z[label]) : 0.f, s, top);
+}
+
+template <int DT, int K>
+__global__ __launch_bounds__(256) void tile_bwd_kernel(const Args a, const int stride) {
+    typedef Elem<DT> E;
+    extern __shared__ __attribute__((aligned(16))) char tile[];
+    const dsaspp_scores_desc& d = a.d;
+    const int V = d.n_class;
+    const int64_t row0 = (int64_t)blockIdx.x * TILE_ROWS, row = row0 + threadIdx.x;
+    const int n = a.rows - row0 < TILE_ROWS ? (int)(a.rows - row0) : TILE_ROWS;
+    copy_tile<DT, false>(tile, const_cast<typename E::T*>(reinterpret_cast<const typename E::T*>(d.logits)) + row0 * V, n * V, V, stride);
+    Up<K> u[1];
+    if ((int)threadIdx.x < n) {
+        const Row r = row_of(a, row);
+        load_up<K, 1>(d, a.plane, row, r.i0, r.rem, 1, u);
+    }
+    __syncthreads();
+    if ((int)threadIdx.x < n) {
+        typename E::T* z = reinterpret_cast<typename E::T*>(tile + threadIdx.x * stride);
+#pragma unroll 4
+        for (int c = 0; c < V; ++c) z[c] = E::down(u[0].grad(E::up(z[c]), c));
+    }
+    __syncthreads();
+    copy_tile<DT, true>(tile, reinterpret_cast<typename E::T*>(d.dlogits) + row0 * V, n * V, V, stride);
+}
+
 // ---------------------------------------------------------------- planes: a lane owns P neighbouring pixels
 // P pixels of one class; np < P only at the end of a row of pixels (lanes past the end hold -inf)
 template <int DT, int P>
@@ -436,7 +547,6 @@ __device__ __forceinline__ void load_px(const typename Elem<DT>::T* p, int np, f
     }
 }
 
-constexpr int PU = 4;                     // classes a lane has in flight
 
 template <int DT, int K, int P>
 __global__ __launch_bounds__(256) void planes_fwd_kernel(const Args a, const int64_t groups, const int64_t per_row) {
@@ -500,9 +610,21 @@ __global__ __launch_bounds__(256) void planes_fwd_kernel(const Args a, const int
             store_row<P>(d.entropy + row, np, o);
         }
         if (d.stats) {
+            float lo[P], hi[P];           // (m, log s) pairs of the first and the second half of the pixels
 #pragma unroll
-            for (int q = 0; q < P; ++q)
-                if (q < np) store_stats(d.stats, row + q, s[q], log_s[q]);
+            for (int q = 0; q < P; ++q) {
+                float* half = 2 * q < P ? lo : hi;
+                half[2 * q % P] = s[q].empty() ? 0.f : s[q].m;
+                if (P > 1) half[(2 * q + 1) % P] = s[q].empty() ? INFINITY : log_s[q];
+            }
+            if (P > 1 && np == P) {
+                store_row<P>(d.stats + 2 * row, P, lo);
+                store_row<P>(d.stats + 2 * row + P, P, hi);
+            } else {
+#pragma unroll
+                for (int q = 0; q < P; ++q)
+                    if (q < np) store_stats(d.stats, row + q, s[q], log_s[q]);
+            }
         }
 #pragma unroll
         for (int j = 0; j < K; ++j)
@@ -541,7 +663,7 @@ __global__ __launch_bounds__(256) void planes_bwd_kernel(const Args a, const int
 #pragma unroll
             for (int q = 0; q < P; ++q) f[q] = u[q].grad(f[q], c);
             typename E::T* oc = o + c * a.plane;
-            if (P > 1 && np == P) {
+            if (P == 4 && np == P) {
                 typename E::V4 w;
 #pragma unroll
                 for (int q = 0; q < 4; ++q) w[q] = E::down(f[q < P ? q : 0]);
@@ -574,28 +696,27 @@ int check(const dsaspp_scores_desc* d, const char* who, Args* a) {
 
 unsigned grid_for(int64_t blocks) { return (unsigned)(blocks < (1 << 20) ? blocks : (1 << 20)); }
 
-// Pixels per lane: 4 where they are contiguous and there are enough of them to fill the chip (256 CUs of 8 waves) all the same.
-int px_per_lane(const Args& a) { return a.d.s2 == 1 && a.d.d2 >= 4 && a.rows >= 4 * 256 * 512 ? 4 : 1; }
+// Pixels per lane: 4 where they are contiguous and there are enough of them to fill the chip (256 CUs of 8 waves) all the same.  8 pixels
+// of a 16-bit type per lane were slower at every top_k (19 classes: 32 against 30 us without alternatives, 78 against 60 us with 3).
+int px_per_lane(const Args& a) { return (a.d.s2 == 1 || a.d.d2 == 1) && a.d.d2 >= 4 && a.rows >= 4 * 256 * 512 ? 4 : 1; }
 
 template <int DT, int K, bool BWD>
 void launch_planes(const Args& a, hipStream_t s) {
     const int P = px_per_lane(a);
     const int64_t per_row = (a.d.d2 + P - 1) / P, groups = a.d.d0 * a.d.d1 * per_row;
     const dim3 grid(grid_for((groups + 255) / 256)), block(256);
-    if (BWD) {
-        if (P == 4) hipLaunchKernelGGL((planes_bwd_kernel<DT, K, 4>), grid, block, 0, s, a, groups, per_row);
-        else hipLaunchKernelGGL((planes_bwd_kernel<DT, K, 1>), grid, block, 0, s, a, groups, per_row);
-    } else {
-        if (P == 4) hipLaunchKernelGGL((planes_fwd_kernel<DT, K, 4>), grid, block, 0, s, a, groups, per_row);
-        else hipLaunchKernelGGL((planes_fwd_kernel<DT, K, 1>), grid, block, 0, s, a, groups, per_row);
-    }
+#define LAUNCH(P) \
+    if constexpr (BWD) hipLaunchKernelGGL((planes_bwd_kernel<DT, K, P>), grid, block, 0, s, a, groups, per_row); \
+    else hipLaunchKernelGGL((planes_fwd_kernel<DT, K, P>), grid, block, 0, s, a, groups, per_row)
+    if (P == 4) { LAUNCH(4); } else { LAUNCH(1); }
+#undef LAUNCH
 }
 
 template <int DT, int K, int TPR, bool BWD>
 void launch_rows_tpr(const Args& a, hipStream_t s) {
     constexpr int T = BWD && TPR > 256 ? 256 : TPR, BLOCK = T > 256 ? T : 256, RPB = BLOCK / T;
     const dim3 grid(grid_for((a.rows + RPB - 1) / RPB)), block(BLOCK);
-    if (BWD) hipLaunchKernelGGL((rows_bwd_kernel<DT, K, T>), grid, block, 0, s, a);
+    if constexpr (BWD) hipLaunchKernelGGL((rows_bwd_kernel<DT, K, T>), grid, block, 0, s, a);
     else hipLaunchKernelGGL((rows_fwd_kernel<DT, K, TPR>), grid, block, 0, s, a);
 }
 
@@ -615,17 +736,32 @@ int part_span(const dsaspp_scores_desc& d, int parts) {        // classes of a p
 // Lanes per row: 4 hold the lane butterflies and the ends of rows cheap (150 classes: 32 us with 4, 57 with 16, 183 with 64 for 223729 rows);
 // more only as long as the rows are too few to fill the chip, and every lane keeps a vector (1203 classes, 8191 rows: 41 us with 4,
 // 14 with 16, 12 with 64, 20 with 256).
+//
+// The backward pass joins nothing, and its writes gain from longer pieces per row: a vector per lane of 16 or 64 wherever there is one
+// (150 classes: 103 us with 16 against 145 with 4; 1203 classes: 88 with 64, 97 with 16 and with 256; forward and backward pass).
 template <int DT, int K, bool BWD>
 void launch_rows(const Args& a, hipStream_t s) {
-    const int64_t vecs = (a.d.n_class + Elem<DT>::N - 1) / Elem<DT>::N;
-    const int parts = BWD ? 1 : row_parts(a.d, a.rows);
-    if (parts > 1) {
-        const int span = part_span(a.d, parts), used = (a.d.n_class + span - 1) / span;
-        hipLaunchKernelGGL((rows_part_kernel<DT, K>), dim3(used, (unsigned)a.rows), dim3(256), 0, s, a, span);
-        hipLaunchKernelGGL((rows_join_kernel<DT, K>), dim3((unsigned)a.rows), dim3(64), 0, s, a, used);
+    const dsaspp_scores_desc& d = a.d;
+    const int size = DT == 1 ? 4 : 2;
+    const bool dense = (d.d2 == 1 || d.s2 == d.n_class) && (d.d1 == 1 || d.s1 == d.d2 * d.n_class) && (d.d0 == 1 || d.s0 == a.plane * d.n_class);
+    if (dense && d.n_class * size <= TILE_ROW_BYTES && a.rows >= 16 * TILE_ROWS && a.rows < ((int64_t)TILE_ROWS << 30)) {
+        const int stride = d.n_class * size + (d.n_class % 8 == 0 ? 16 : 0);
+        const dim3 grid((unsigned)((a.rows + TILE_ROWS - 1) / TILE_ROWS)), block(TILE_ROWS);
+        if constexpr (BWD) hipLaunchKernelGGL((tile_bwd_kernel<DT, K>), grid, block, TILE_ROWS * stride, s, a, stride);
+        else hipLaunchKernelGGL((tile_fwd_kernel<DT, K>), grid, block, TILE_ROWS * stride, s, a, stride);
         return;
     }
-    int tpr = 4;
+    if constexpr (!BWD) {
+        const int parts = row_parts(a.d, a.rows);
+        if (parts > 1) {
+            const int span = part_span(a.d, parts), used = (a.d.n_class + span - 1) / span;
+            hipLaunchKernelGGL((rows_part_kernel<DT, K>), dim3(used, (unsigned)a.rows), dim3(256), 0, s, a, span);
+            hipLaunchKernelGGL((rows_join_kernel<DT, K>), dim3((unsigned)a.rows), dim3(64), 0, s, a, used);
+            return;
+        }
+    }
+    const int64_t vecs = (d.n_class + Elem<DT>::N - 1) / Elem<DT>::N;
+    int tpr = BWD ? (vecs >= 128 ? 64 : vecs >= 16 ? 16 : 4) : 4;
     while (tpr < 1024 && tpr * 4 <= vecs && a.rows * tpr < 256 * 1024) tpr *= 4;
     if (tpr == 4) launch_rows_tpr<DT, K, 4, BWD>(a, s);
     else if (tpr == 16) launch_rows_tpr<DT, K, 16, BWD>(a, s);
@@ -641,6 +777,7 @@ void launch_k(const Args& a, int k, hipStream_t s) {
     if (k == 0) LAUNCH(0);
     else if (k == 1) LAUNCH(1);
     else if (k <= 3) LAUNCH(3);
+    else if (k <= 5) LAUNCH(5);
     else LAUNCH(8);
 #undef LAUNCH
 }

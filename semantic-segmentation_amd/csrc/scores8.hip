@@ -191,18 +191,6 @@ struct Chain {
 // The K largest of a pixel in the short form.  A key is x with its five lowest bits replaced by the class, so that keeping K + 1
 // keys in order is K + 1 instructions per class (one max, K medians of three) where values and classes apart take 4 K - 1.  Where
 // two neighbours among them are closer than the roundings of x and of the key, the pixel's logits are offered again, exactly.
-// The instructions themselves: the compiler's forms first quieten a key, whose bits might be a signalling NaN for all it knows.
-__device__ __forceinline__ float med3(float a, float b, float c) {
-    float r;
-    asm("v_med3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
-    return r;
-}
-__device__ __forceinline__ float larger(float a, float b) {
-    float r;
-    asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
-    return r;
-}
-
 template <int K>
 struct Keys {
     float v[K + 1];
@@ -338,7 +326,9 @@ __device__ __forceinline__ float row8_sum(float v) {
 // HB: an upstream gradient of the entropy is there.  Per pixel and class  dz = e (k0 + k1 x)  with e = 2^x, x = (z - up) log2 e for
 // any reference up, and per-pixel k0, k1; what falls on the label and on the alternatives is added to lane-private LDS columns instead of
 // being selected by class.
-template <int NC, bool EXACT, bool HB>
+// KT alternatives per pixel pass through registers (0: none have a gradient); MANY: any number of them, read where they are needed.
+constexpr int MANY = -1;
+template <int NC, bool EXACT, bool HB, int KT>
 __global__ __launch_bounds__(256, NC <= 19 ? 3 : 1) void scores8_bwd_kernel(const dsaspp_scores8_desc d, const int tiles_x, const int tiles_y) {
     constexpr int CS = NC | 1, CELLS = TCX * TCY, KS = CELLS * CS;
     __shared__ float corner[PX * PY * CS];
@@ -380,7 +370,27 @@ __global__ __launch_bounds__(256, NC <= 19 ? 3 : 1) void scores8_bwd_kernel(cons
             const float a = label >= 0 ? in.a : 0.f, b = in.b;
             float A = a;
             bool live = a != 0.f || b != 0.f;
-            if (d.g_top)
+            constexpr int KR = KT > 0 ? KT : 1;
+            float gt[KR];
+            int64_t ct_[KR];                          // classes of the alternatives: asked for now, needed after the row's arithmetic
+            if (KT > 0) {
+#pragma unroll
+                for (int j = 0; j < KR; ++j) {
+                    gt[j] = 0.f;
+                    ct_[j] = -1;
+                    if (j < d.top_k) {
+                        const int64_t o = at + ((int64_t)tl.n * (d.top_k - 1) + j) * plane;
+                        gt[j] = d.g_top_one ? d.g_top[0] : (d.g_top + o)[X];
+                        ct_[j] = (d.top_class + o)[X];
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < KR; ++j) {
+                    live = live || gt[j] != 0.f;
+                    A += brief || ct_[j] >= 0 ? gt[j] : 0.f;      // in the short form every pixel has its alternatives
+                }
+            }
+            if (KT == MANY)
                 for (int j = 0; j < d.top_k; ++j) {
                     const int64_t o = at + ((int64_t)tl.n * (d.top_k - 1) + j) * plane;
                     const float g = d.g_top_one ? d.g_top[0] : (d.g_top + o)[X];
@@ -444,7 +454,15 @@ __global__ __launch_bounds__(256, NC <= 19 ? 3 : 1) void scores8_bwd_kernel(cons
                 o0[0] += a * hy;
                 o0[NC * 256] += a * ly;
             }
-            if (d.g_top)
+            if (KT > 0) {
+#pragma unroll
+                for (int j = 0; j < KR; ++j)
+                    if (ct_[j] >= 0 && ct_[j] < nc) {
+                        oh[(int)ct_[j] * 256 + tid] += gt[j] * hy;
+                        oh[(NC + (int)ct_[j]) * 256 + tid] += gt[j] * ly;
+                    }
+            }
+            if (KT == MANY)
                 for (int j = 0; j < d.top_k; ++j) {
                     const int64_t o = at + ((int64_t)tl.n * (d.top_k - 1) + j) * plane;
                     const int64_t tc = (d.top_class + o)[X];
@@ -572,14 +590,25 @@ void launch_fwd(const dsaspp_scores8_desc& d, int tx, int ty, unsigned grid, hip
     if (d.top_k == 0) LAUNCH(0);
     else if (d.top_k == 1) LAUNCH(1);
     else if (d.top_k <= 3) LAUNCH(3);
+    else if (d.top_k <= 5) LAUNCH(5);
     else LAUNCH(8);
 #undef LAUNCH
 }
 
 template <int NC, bool EX>
 void launch_bwd(const dsaspp_scores8_desc& d, int tx, int ty, unsigned grid, hipStream_t s) {
-    if (d.g_entropy) hipLaunchKernelGGL((scores8_bwd_kernel<NC, EX, true>), dim3(grid), dim3(256), 0, s, d, tx, ty);
-    else hipLaunchKernelGGL((scores8_bwd_kernel<NC, EX, false>), dim3(grid), dim3(256), 0, s, d, tx, ty);
+#define LAUNCH(HB, KT) hipLaunchKernelGGL((scores8_bwd_kernel<NC, EX, HB, KT>), dim3(grid), dim3(256), 0, s, d, tx, ty)
+    const int k = d.g_top ? d.top_k : 0;
+    if (d.g_entropy) {
+        if (k == 0) LAUNCH(true, 0);
+        else if (k <= 3) LAUNCH(true, 3);
+        else LAUNCH(true, MANY);
+    } else {
+        if (k == 0) LAUNCH(false, 0);
+        else if (k <= 3) LAUNCH(false, 3);
+        else LAUNCH(false, MANY);
+    }
+#undef LAUNCH
 }
 
 }  // namespace

@@ -90,6 +90,19 @@ struct Soft {
     }
 };
 
+// The instructions themselves: the compiler's forms first quieten their operands, whose bits might be a signalling NaN for all it
+// knows.  (A row with a NaN gives no list: whatever the instructions make of it is not used.)
+__device__ __forceinline__ float med3(float a, float b, float c) {
+    float r;
+    asm("v_med3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+__device__ __forceinline__ float larger(float a, float b) {
+    float r;
+    asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+    return r;
+}
+
 // The K largest, descending; offered in ascending class order, so that of equal ones the lowest class stays in front.
 template <int K>
 struct Top {
@@ -106,11 +119,11 @@ struct Top {
 #pragma unroll
         for (int j = K - 1; j > 0; --j) {
             i[j] = g[j - 1] ? i[j - 1] : (g[j] ? c : i[j]);
-            v[j] = g[j - 1] ? v[j - 1] : (g[j] ? z : v[j]);
+            v[j] = med3(v[j - 1], v[j], z);
         }
         if (K > 0) {
             i[0] = g[0] ? c : i[0];
-            v[0] = g[0] ? z : v[0];
+            v[0] = larger(v[0], z);
         }
     }
     // The K largest of the lists of LANES neighbouring lanes, in every one of them: K times the best head, whose lane moves up.

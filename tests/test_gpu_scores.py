@@ -123,6 +123,17 @@ def test_rows_of_classes(classes, dtype):
         _check(z, labels, logits, k, True)
 
 
+@pytest.mark.parametrize('shape', [(4096, 2), (4097, 3), (5000, 9), (4351, 16), (4352, 19), (4353, 32), (4500, 33), (4200, 40), (4100, 63), (4400, 64),
+                                   (3, 19, 40, 41), (2, 24, 53, 47)])
+@pytest.mark.parametrize('dtype', list(DT))
+def test_many_rows_of_few_classes(shape, dtype):
+    z, labels, logits = _make(shape, DT[dtype], 'last', shape[1])
+    for k in (0, 2):
+        _check(z, labels, logits, k, True)
+    z, labels, logits = _make(shape, DT[dtype], 'last', shape[1], mask='rows')
+    _check(z, labels, logits, min(8, shape[1]), True)
+
+
 @pytest.mark.parametrize('rows,classes', [(1, 5003), (3, 8193), (2, 21841), (1030, 8195), (1, 4096), (1, 100001), (127, 16385), (128, 16385), (20, 4099)])
 @pytest.mark.parametrize('dtype', ['fp32', 'bf16'])
 def test_long_rows(rows, classes, dtype):

@@ -326,10 +326,11 @@ __device__ __forceinline__ float row8_sum(float v) {
 // HB: an upstream gradient of the entropy is there.  Per pixel and class  dz = e (k0 + k1 x)  with e = 2^x, x = (z - up) log2 e for
 // any reference up, and per-pixel k0, k1; what falls on the label and on the alternatives is added to lane-private LDS columns instead of
 // being selected by class.
-// KT alternatives per pixel pass through registers (0: none have a gradient); MANY: any number of them, read where they are needed.
-constexpr int MANY = -1;
+// KT (0, 3 or 8): room for the gradients of a pixel's alternatives.  All are asked for before the first is used, one by one they cost a
+// trip to memory each, twice per row (five alternatives, three 1024 x 2048 pictures, forward and backward: 493 us against 350).
+// With eight and an entropy gradient two waves per SIMD without spills are faster than three with (350 against 535 us).
 template <int NC, bool EXACT, bool HB, int KT>
-__global__ __launch_bounds__(256, NC <= 19 ? 3 : 1) void scores8_bwd_kernel(const dsaspp_scores8_desc d, const int tiles_x, const int tiles_y) {
+__global__ __launch_bounds__(256, NC <= 19 ? (HB && KT == 8 ? 2 : 3) : 1) void scores8_bwd_kernel(const dsaspp_scores8_desc d, const int tiles_x, const int tiles_y) {
     constexpr int CS = NC | 1, CELLS = TCX * TCY, KS = CELLS * CS;
     __shared__ float corner[PX * PY * CS];
     __shared__ float oh[2 * NC * 256];                // [corner row][class][lane]
@@ -371,32 +372,24 @@ __global__ __launch_bounds__(256, NC <= 19 ? 3 : 1) void scores8_bwd_kernel(cons
             float A = a;
             bool live = a != 0.f || b != 0.f;
             constexpr int KR = KT > 0 ? KT : 1;
+            constexpr bool EARLY = KT <= 3;           // their classes too: eight would not fit beside the row's arithmetic
             float gt[KR];
-            int64_t ct_[KR];                          // classes of the alternatives: asked for now, needed after the row's arithmetic
+            int64_t ct_[KR];
+            auto load_classes = [&]() {
+#pragma unroll
+                for (int j = 0; j < KR; ++j) ct_[j] = j < d.top_k ? (d.top_class + at + ((int64_t)tl.n * (d.top_k - 1) + j) * plane)[X] : -1;
+            };
             if (KT > 0) {
 #pragma unroll
-                for (int j = 0; j < KR; ++j) {
-                    gt[j] = 0.f;
-                    ct_[j] = -1;
-                    if (j < d.top_k) {
-                        const int64_t o = at + ((int64_t)tl.n * (d.top_k - 1) + j) * plane;
-                        gt[j] = d.g_top_one ? d.g_top[0] : (d.g_top + o)[X];
-                        ct_[j] = (d.top_class + o)[X];
-                    }
-                }
+                for (int j = 0; j < KR; ++j)
+                    gt[j] = j >= d.top_k ? 0.f : d.g_top_one ? d.g_top[0] : (d.g_top + at + ((int64_t)tl.n * (d.top_k - 1) + j) * plane)[X];
+                if (EARLY || !brief) load_classes();
 #pragma unroll
                 for (int j = 0; j < KR; ++j) {
                     live = live || gt[j] != 0.f;
                     A += brief || ct_[j] >= 0 ? gt[j] : 0.f;      // in the short form every pixel has its alternatives
                 }
             }
-            if (KT == MANY)
-                for (int j = 0; j < d.top_k; ++j) {
-                    const int64_t o = at + ((int64_t)tl.n * (d.top_k - 1) + j) * plane;
-                    const float g = d.g_top_one ? d.g_top[0] : (d.g_top + o)[X];
-                    live = live || g != 0.f;
-                    if ((d.top_class + o)[X] >= 0) A += g;
-                }
             // the label's sums are read now and written back after the row's arithmetic
             float* const o0 = oh + max(label, 0) * 256 + tid;
             const float w0 = o0[0], w1 = o0[NC * 256];
@@ -455,6 +448,7 @@ __global__ __launch_bounds__(256, NC <= 19 ? 3 : 1) void scores8_bwd_kernel(cons
                 o0[NC * 256] += a * ly;
             }
             if (KT > 0) {
+                if (!EARLY) load_classes();
 #pragma unroll
                 for (int j = 0; j < KR; ++j)
                     if (ct_[j] >= 0 && ct_[j] < nc) {
@@ -462,16 +456,6 @@ __global__ __launch_bounds__(256, NC <= 19 ? 3 : 1) void scores8_bwd_kernel(cons
                         oh[(NC + (int)ct_[j]) * 256 + tid] += gt[j] * ly;
                     }
             }
-            if (KT == MANY)
-                for (int j = 0; j < d.top_k; ++j) {
-                    const int64_t o = at + ((int64_t)tl.n * (d.top_k - 1) + j) * plane;
-                    const int64_t tc = (d.top_class + o)[X];
-                    if (tc >= 0 && tc < nc) {
-                        const float g = d.g_top_one ? d.g_top[0] : (d.g_top + o)[X];
-                        oh[(int)tc * 256 + tid] += g * hy;
-                        oh[(NC + (int)tc) * 256 + tid] += g * ly;
-                    }
-                }
         }
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
@@ -602,11 +586,11 @@ void launch_bwd(const dsaspp_scores8_desc& d, int tx, int ty, unsigned grid, hip
     if (d.g_entropy) {
         if (k == 0) LAUNCH(true, 0);
         else if (k <= 3) LAUNCH(true, 3);
-        else LAUNCH(true, MANY);
+        else LAUNCH(true, 8);
     } else {
         if (k == 0) LAUNCH(false, 0);
         else if (k <= 3) LAUNCH(false, 3);
-        else LAUNCH(false, MANY);
+        else LAUNCH(false, 8);
     }
 #undef LAUNCH
 }

@@ -59,6 +59,15 @@ def test_sizes_and_types(dtypes, kind):
     _check_clip(ts, 0.25 * _norm(ts, kind), kind)
 
 
+@pytest.mark.parametrize('sizes', [[1], [8192], [8193], [1, 2, 3, 4, 5, 6, 7], [1000] * 8, [1000] * 9, [4096, 4096], [4096, 4097]])
+@pytest.mark.parametrize('dtypes', [(F32,), (B16,), (F16, F32)])
+@pytest.mark.parametrize('kind', [2.0, math.inf])
+def test_few_elements(sizes, dtypes, kind):
+    ts = _tensors(sizes, dtypes, sum(sizes))
+    _check_clip(ts, 0.3 * _norm(ts, kind), kind)
+    _check_clip(ts, 2.0 * _norm(ts, kind), kind)
+
+
 @pytest.mark.parametrize('n', [1, 5, 8192, 8193, 3_000_001])
 @pytest.mark.parametrize('dtype', [F32, B16])
 def test_one_tensor(n, dtype):

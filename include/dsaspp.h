@@ -567,7 +567,8 @@ int dsaspp_preprocess(const dsaspp_prep_desc* d, dsaspp_stream_t stream);
  * Rows are numbered (i0, i1, i2) row-major over [d0][d1][d2]; logits of row (i0, i1, i2), class c at
  * logits[i0*s0 + i1*s1 + i2*s2 + c*sc] (strides in elements, >= 0).  labels, logp and entropy are dense [rows];
  * top_logp and top_class are [d0][top_k][d1][d2].  dlogits is dense: [rows][n_class] when sc == 1, else [d0][n_class][d1][d2].
- * Arithmetic is fp32 on logits of any dtype; dlogits has the logits' dtype (0 = bf16, 1 = fp32, 2 = fp16), rounded once. */
+ * Arithmetic is fp32 on logits of any dtype; dlogits has the logits' dtype (0 = bf16, 1 = fp32, 2 = fp16), rounded once, and must not
+ * overlap the logits. */
 #define DSASPP_SCORES_MAX_TOP 8
 typedef struct dsaspp_scores_desc {
     int32_t dtype, n_class, top_k;
@@ -592,7 +593,9 @@ int dsaspp_scores_bwd(const dsaspp_scores_desc* d, dsaspp_stream_t stream);
 
 /* The same on logits at 1/8 resolution, with the bilinear x8 upsample (align_corners=False) fused in: the full-resolution logits
  * are never written.  z = hy*r0 + ly*r1, r_i = hx*L[yi][x0] + lx*L[yi][x1], every product and sum rounded to fp32 by itself, so the
- * order of the classes is that of those values to the bit.  n_class <= 32.  Logits of image n, pixel (y, x), class c at
+ * order of the classes is that of those values to the bit; what is computed from them carries a few more roundings at the magnitude of
+ * the logits.  A NaN or infinity counts in every pixel whose four source pixels hold it, at weight 0 too, as in torch's upsample.
+ * n_class <= 32, fewer than 2^24 tiles of 64 x 32 pixels.  Logits of image n, pixel (y, x), class c at
  * logits[n*sn + y*sy + x*sx + c*sc]; labels, logp, entropy [n_img][8h][8w]; top_* [n_img][top_k][8h][8w]; upstream gradients
  * likewise.  Backward reads logits, labels and (with g_top) top_class; dlogits at dlogits[n*gn + y*gy + x*gx + c*gc], dtype g_dtype;
  * ws: dsaspp_scores8_workspace floats, contents need not be initialised. */

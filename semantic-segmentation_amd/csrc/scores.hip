@@ -547,7 +547,6 @@ __device__ __forceinline__ void load_px(const typename Elem<DT>::T* p, int np, f
     }
 }
 
-
 template <int DT, int K, int P>
 __global__ __launch_bounds__(256) void planes_fwd_kernel(const Args a, const int64_t groups, const int64_t per_row) {
     typedef Elem<DT> E;
@@ -698,7 +697,7 @@ unsigned grid_for(int64_t blocks) { return (unsigned)(blocks < (1 << 20) ? block
 
 // Pixels per lane: 4 where they are contiguous and there are enough of them to fill the chip (256 CUs of 8 waves) all the same.  8 pixels
 // of a 16-bit type per lane were slower at every top_k (19 classes: 32 against 30 us without alternatives, 78 against 60 us with 3).
-int px_per_lane(const Args& a) { return (a.d.s2 == 1 || a.d.d2 == 1) && a.d.d2 >= 4 && a.rows >= 4 * 256 * 512 ? 4 : 1; }
+int px_per_lane(const Args& a) { return a.d.s2 == 1 && a.d.d2 >= 4 && a.rows >= 4 * 256 * 512 ? 4 : 1; }
 
 template <int DT, int K, bool BWD>
 void launch_planes(const Args& a, hipStream_t s) {
@@ -744,7 +743,7 @@ void launch_rows(const Args& a, hipStream_t s) {
     const dsaspp_scores_desc& d = a.d;
     const int size = DT == 1 ? 4 : 2;
     const bool dense = (d.d2 == 1 || d.s2 == d.n_class) && (d.d1 == 1 || d.s1 == d.d2 * d.n_class) && (d.d0 == 1 || d.s0 == a.plane * d.n_class);
-    if (dense && d.n_class * size <= TILE_ROW_BYTES && a.rows >= 16 * TILE_ROWS && a.rows < ((int64_t)TILE_ROWS << 30)) {
+    if (dense && d.n_class * size <= TILE_ROW_BYTES && a.rows >= 16 * TILE_ROWS && a.rows < (1ll << 31)) {      // a lane per row: a grid has fewer than 2^32 lanes
         const int stride = d.n_class * size + (d.n_class % 8 == 0 ? 16 : 0);
         const dim3 grid((unsigned)((a.rows + TILE_ROWS - 1) / TILE_ROWS)), block(TILE_ROWS);
         if constexpr (BWD) hipLaunchKernelGGL((tile_bwd_kernel<DT, K>), grid, block, TILE_ROWS * stride, s, a, stride);

@@ -426,8 +426,8 @@ __global__ __launch_bounds__(256, NC <= 19 ? (HB && KT == 8 ? 2 : 3) : 1) void s
                 s.clear();
 #pragma unroll 1
                 for (int c = 0; c < nc; ++c) s.m = fmaxf(s.m, q.plain_logit(corner, c, hy, ly));
-    #pragma unroll 1
-            for (int c = 0; c < nc; ++c) s.add(q.plain_logit(corner, c, hy, ly));
+#pragma unroll 1
+                for (int c = 0; c < nc; ++c) s.add(q.plain_logit(corner, c, hy, ly));
                 if (s.empty()) continue;              // every class masked out
                 const float inv = 1.f / s.s, k1 = HB ? -b * SR_LN2 * inv : 0.f, k0 = HB ? -A * inv - k1 * (s.t * inv) : -A * inv;
 #pragma unroll 1
@@ -559,7 +559,7 @@ int check(const dsaspp_scores8_desc* d, const char* who, int* tx, int* ty, int64
     *tx = (d->w + 1 + TCX - 1) / TCX;
     *ty = (d->h + 1 + TCY - 1) / TCY;
     *tiles = (int64_t)d->n_img * *tx * *ty;
-    DS_REQUIRE(*tiles < (1ll << 31), "%s: too many pixels", who);
+    DS_REQUIRE(*tiles < (1ll << 24), "%s: too many pixels for one launch (fewer than 2^32 lanes)", who);
     return 0;
 }
 

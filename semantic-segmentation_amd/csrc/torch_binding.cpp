@@ -9,6 +9,7 @@
 
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/VirtualGuardImpl.h>
 #include <pybind11/pybind11.h>
 #include <pybind11/stl.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -118,7 +119,7 @@ c10::intrusive_ptr<Plan> make_plan(at::IntArrayRef shape, at::Device device, con
     if (labels.has_value()) {
         VALUE_CHECK(labels->scalar_type() == at::kLong && labels->sizes() == at::IntArrayRef(p->rows) && labels->device() == device,
                     "labels must be an int64 tensor of shape %s on the device of the logits", shape_text(p->rows).c_str());
-        p->labels = labels->contiguous();
+        p->labels = labels->contiguous().resolve_neg();
     }
     p->top_k = (int)top_k;
     p->ignore_index = ignore_index;
@@ -225,7 +226,7 @@ Out scores_forward(const Plan& p, Tensor logits, bool need_stats) {
 // An upstream gradient for the kernels: dense, or one value for all (what sum() and mean() send back).
 Tensor upstream(const Tensor& g, const float*& at, int32_t& one) {
     if (!g.defined()) return g;
-    Tensor t = g.scalar_type() == at::kFloat ? g : g.to(at::kFloat);
+    Tensor t = (g.scalar_type() == at::kFloat ? g : g.to(at::kFloat)).resolve_neg();
     one = 1;
     for (int64_t i = 0; i < t.dim(); ++i)
         if (t.stride(i) != 0 && t.size(i) != 1) one = 0;
@@ -290,6 +291,20 @@ Tensor differentiable_once(Tensor g) {
     return (*err)(torch::autograd::variable_list{v})[0];
 }
 
+// A leaf's gradient accumulator keeps the stream of the oldest live graph that reaches it.  If that is not the stream being captured,
+// handing it a gradient would pull a stream that is not captured into the graph, which ends the process: refused here, before it happens.
+void check_capture(const Tensor& logits) {
+    if (!logits.is_leaf() || !logits.requires_grad()) return;
+    const auto acc = torch::autograd::impl::try_get_grad_accumulator(logits);
+    const auto stream = acc ? acc->stream() : std::nullopt;
+    if (!stream || *stream == c10::impl::VirtualGuardImpl(logits.device().type()).getStream(logits.device())) return;
+    const c10::DeviceGuard guard(logits.device());
+    const py::gil_scoped_acquire gil;
+    if (py::module_::import("torch.cuda").attr("is_current_stream_capturing")().cast<bool>())
+        throw std::runtime_error("label_scores: a backward pass is captured while a graph made on another stream still holds the same logits: "
+                                 "drop that graph first, or detach the logits for the capture");
+}
+
 struct LabelScores : torch::autograd::Function<LabelScores> {
     static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& logits, c10::intrusive_ptr<Plan> plan) {
         const Out o = scores_forward(*plan, logits, true);
@@ -305,6 +320,7 @@ struct LabelScores : torch::autograd::Function<LabelScores> {
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list g) {
         const auto saved = ctx->get_saved_variables();
+        check_capture(saved[0]);
         const auto holder = ctx->saved_data["plan"].toCapsule();
         const Plan& p = *static_cast<Plan*>(holder.get());
         size_t k = 0;
@@ -320,9 +336,10 @@ struct LabelScores : torch::autograd::Function<LabelScores> {
 
 py::object opt(const Tensor& t) { return t.defined() ? py::cast(t) : py::none(); }
 
-py::tuple label_scores(const Tensor& logits, const OptTensor& labels, int64_t top_k, int64_t ignore_index, bool entropy, int64_t upsample, int64_t stream) {
-    TYPE_CHECK(dtype_code(logits.scalar_type()) >= 0 && logits.layout() == at::kStrided, "logits must be a float32, bfloat16 or float16 tensor, got %s",
-               dtype_name(logits).c_str());
+py::tuple label_scores(const Tensor& given, const OptTensor& labels, int64_t top_k, int64_t ignore_index, bool entropy, int64_t upsample, int64_t stream) {
+    TYPE_CHECK(dtype_code(given.scalar_type()) >= 0 && given.layout() == at::kStrided, "logits must be a float32, bfloat16 or float16 tensor, got %s",
+               dtype_name(given).c_str());
+    const Tensor logits = given.resolve_neg();        // itself, unless it is a view that torch negates when it is read
     auto p = make_plan(logits.sizes(), logits.device(), labels, top_k, ignore_index, entropy, upsample);
     p->stream = stream;
     Out o;
@@ -453,8 +470,8 @@ Grads gather(const py::list& list, bool of_parameters, const char* who) {
 
 Tensor grad_norm(const py::list& grads, double norm_type, int64_t stream) {
     Grads g = gather(grads, false, "grad_norm");
-    if (g.tensors.empty()) return at::zeros({}, at::kFloat);
     g.set_norm_type(norm_type, "grad_norm");
+    if (g.tensors.empty()) return at::zeros({}, at::kFloat);
     const c10::DeviceGuard guard(g.device);
     g.ready(false, "grad_norm");
     call(api.grad_norm_partials(&g.d, handle(stream)));
@@ -490,7 +507,7 @@ Tensor clip_grads(const py::list& grads, bool of_parameters, double max_norm, do
 Tensor adam_update(const Tensor& p, const Tensor& grad, const Tensor& m, const Tensor& v, int64_t step, double lr, double beta1, double beta2, double eps,
                    double weight_decay, double grad_scale, double max_grad_norm, double norm_type, const OptTensor& shadow, int64_t stream) {
     for (const Tensor* t : {&p, &grad, &m, &v})
-        VALUE_CHECK(t->is_cuda() && t->scalar_type() == at::kFloat && t->numel() == p.numel() && t->device() == p.device() && t->is_contiguous(),
+        VALUE_CHECK(t->is_cuda() && t->scalar_type() == at::kFloat && t->numel() == p.numel() && t->device() == p.device() && t->is_contiguous() && !t->is_neg(),
                     "adam_update_ needs contiguous float32 tensors of one size on one GPU");
     if (shadow.has_value())
         VALUE_CHECK(shadow->scalar_type() == at::kBFloat16 && shadow->numel() == p.numel() && shadow->device() == p.device() && shadow->is_contiguous(),

@@ -458,6 +458,63 @@ def test_captured_and_replayed(shape, upsample):
                 assert torch.equal(a, b)
 
 
+def test_capture_beside_a_live_graph_of_the_same_leaf_is_refused(monkeypatch):
+    """The accumulator of a leaf belongs to the stream of the graph that made it: asked whether that is seen, without a real capture."""
+    leaf = torch.randn(4, 5, device='cuda', requires_grad=True)
+    alive = _label_scores(leaf)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        g = torch.ones(4, device='cuda')
+        want, = torch.autograd.grad(_label_scores(leaf).entropy, leaf, g)
+        s = _label_scores(leaf)
+        with monkeypatch.context() as m:
+            m.setattr(torch.cuda, 'is_current_stream_capturing', lambda: True)
+            with pytest.raises(RuntimeError, match='captured'):
+                torch.autograd.grad(s.entropy, leaf, g)
+            del alive, s
+            got, = torch.autograd.grad(_label_scores(leaf).entropy, leaf, g)       # the side stream's own graph
+            twice = leaf * 2.0
+            torch.autograd.grad(_label_scores(twice).entropy, twice, g)
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+
+
+def test_views_that_are_negated_when_read():
+    z = torch.randn(6, 19, 5, 4, device='cuda')
+    labels = torch.randint(0, 19, (6, 5, 4), device='cuda')
+    a, b = z.clone().requires_grad_(), z.clone().requires_grad_()
+    s, t = _label_scores(torch._neg_view(a), torch._neg_view(-labels), top_k=2), _label_scores(-b, labels, top_k=2)
+    for x, y in zip(s, t):
+        assert torch.equal(x, y)
+    g = torch.randn(6, 5, 4, device='cuda')
+    s.logp.backward(torch._neg_view(g))
+    t.logp.backward(-g)
+    assert torch.equal(a.grad, b.grad)
+
+
+def test_more_rows_than_a_grid_has_lanes():
+    """2^32 + 300 rows of 2 classes (17 GB): a lane per row no longer is one launch."""
+    n = 2 ** 32 + 300
+    logits = torch.zeros((n, 2), dtype=torch.bfloat16, device='cuda')
+    logits[-3:] = torch.tensor([[1.0, -1.0], [0.5, 0.0], [-math.inf, -math.inf]], dtype=torch.bfloat16)
+    logits.requires_grad_()
+    s = _label_scores(logits)
+    g = torch.ones((), device='cuda').expand(n)
+    grad, = torch.autograd.grad(s.entropy, logits, g)
+    with torch.no_grad():
+        flat = s.entropy[:-3]
+        assert abs(float(flat.min()) - math.log(2)) < 1e-6 and float(flat.max()) == float(flat.min())
+        assert not bool(grad[:-3].any()) and not bool(grad[-1].any())
+        tail = logits[-3:].detach().cpu().double()
+        p = torch.softmax(tail[:2], 1)
+        h = -(p * p.log()).sum(1)
+        assert torch.allclose(s.entropy[-3:-1].cpu().double(), h, rtol=0, atol=8 * R.U)
+        assert float(s.entropy[-1]) == 0.0
+        want = -p * (p.log() + h[:, None])
+        assert torch.allclose(grad[-3:-1].cpu().double(), want, rtol=2.0 ** -8, atol=8 * R.U)
+
+
 def test_second_derivative_is_refused():
     logits = torch.randn(4, 5, device='cuda', requires_grad=True)
     s = _label_scores(logits)

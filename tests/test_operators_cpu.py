@@ -67,6 +67,7 @@ def _scores8(**k):
 
 @pytest.mark.parametrize('bad,message', [
     (dict(n_class=33), 'n_class'), (dict(h=0), 'geometry'), (dict(w=1 << 20), 'geometry'), (dict(n_img=1 << 30, h=1000, w=1000), 'too many'),
+    (dict(n_img=1 << 24, h=1, w=1), 'too many'),
     (dict(top_k=9), 'top_k'), (dict(logits=GOOD + 1), 'aligned'), (dict(sx=-1), 'stride'), (dict(labels=None), 'labels'), (dict(logp=None), 'nothing')])
 def test_scores8_forward_descriptor(bad, message):
     assert _lib.load().dsaspp_scores8_fwd(ctypes.byref(_scores8(**bad)), None) != 0

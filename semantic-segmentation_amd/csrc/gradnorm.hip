@@ -14,7 +14,7 @@
 
 namespace {
 
-constexpr int CHUNK = 8192;               // elements of one range that a block takes at a time
+constexpr int CHUNK = 4096;               // elements of one range that a block takes at a time
 constexpr int MAX_BLOCKS = 2048;          // 8 blocks of 4 waves per CU fill the chip; a block takes several chunks in a row
 // The ranges of one launch travel in its kernel arguments (4.0 of 4 KB), ten bytes each: 32 bits of distance from the first range, in
 // elements, 32 bits of length and 16 bits of first chunk.  24 bytes each made three launches of what fits one; a launch costs the host 3 us.

@@ -597,7 +597,7 @@ int dsaspp_scores_bwd(const dsaspp_scores_desc* d, dsaspp_stream_t stream);
  * the logits.  A NaN or infinity counts in every pixel whose four source pixels hold it, at weight 0 too, as in torch's upsample.
  * n_class <= 32, fewer than 2^24 tiles of 64 x 32 pixels.  Logits of image n, pixel (y, x), class c at
  * logits[n*sn + y*sy + x*sx + c*sc]; labels, logp, entropy [n_img][8h][8w]; top_* [n_img][top_k][8h][8w]; upstream gradients
- * likewise.  Backward reads logits, labels and (with g_top) top_class; dlogits at dlogits[n*gn + y*gy + x*gx + c*gc], dtype g_dtype;
+ * likewise.  Backward reads logits, labels, stats and (with g_entropy) entropy and (with g_top) top_class; dlogits at dlogits[n*gn + y*gy + x*gx + c*gc], dtype g_dtype;
  * ws: dsaspp_scores8_workspace floats, contents need not be initialised. */
 typedef struct dsaspp_scores8_desc {
     int32_t n_img, h, w, n_class, top_k;
@@ -607,6 +607,7 @@ typedef struct dsaspp_scores8_desc {
     const int64_t* labels;
     int64_t ignore_index;
     float* logp; float* entropy; float* top_logp; int64_t* top_class;
+    float* stats;             /* [n_img][8h][8w] for the backward call: sum of exponentials relative to a reference that it forms again */
     const float* g_logp; const float* g_entropy; const float* g_top;
     int32_t g_logp_one, g_entropy_one, g_top_one;
     void* dlogits;

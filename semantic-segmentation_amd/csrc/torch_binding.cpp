@@ -190,9 +190,9 @@ Out scores_forward(const Plan& p, Tensor logits, bool need_stats) {
         o.top_logp = at::empty(shape, f32);
         o.top_class = at::empty(shape, f32.dtype(at::kLong));
     }
-    if (need_stats && p.upsample == 1) {
+    if (need_stats) {
         std::vector<int64_t> shape = p.rows;
-        shape.push_back(2);
+        if (p.upsample == 1) shape.push_back(2);
         o.stats = at::empty(shape, f32);
     }
     if (p.empty) return o;
@@ -201,6 +201,7 @@ Out scores_forward(const Plan& p, Tensor logits, bool need_stats) {
         d.entropy = ptr<float>(o.entropy);
         d.top_logp = ptr<float>(o.top_logp);
         d.top_class = ptr<int64_t>(o.top_class);
+        d.stats = ptr<float>(o.stats);
     };
     if (p.upsample == 8) {
         dsaspp_scores8_desc d = {};
@@ -211,7 +212,6 @@ Out scores_forward(const Plan& p, Tensor logits, bool need_stats) {
         dsaspp_scores_desc d = {};
         fill_common(d, p, logits);
         outputs(d);
-        d.stats = ptr<float>(o.stats);
         const int64_t need = api.scores_workspace(&d);
         if (need < 0) call(1);
         Tensor ws;
@@ -251,6 +251,7 @@ Tensor scores_backward(const Plan& p, Tensor logits, const Tensor& stats, const 
         fill_common(d, p, logits);
         d.entropy = ptr<float>(entropy);
         d.top_class = ptr<int64_t>(top_class);
+        d.stats = ptr<float>(stats);
         up[0] = upstream(g_logp, d.g_logp, d.g_logp_one);
         up[1] = upstream(g_entropy, d.g_entropy, d.g_entropy_one);
         up[2] = upstream(g_top, d.g_top, d.g_top_one);
@@ -275,7 +276,6 @@ Tensor scores_backward(const Plan& p, Tensor logits, const Tensor& stats, const 
     } else {
         dsaspp_scores_desc d = {};
         inputs(d, up);
-        d.stats = ptr<float>(stats);
         d.dlogits = out.data_ptr();
         call(api.scores_bwd(&d, handle(p.stream)));
     }
@@ -361,20 +361,20 @@ void check_scores(const std::vector<int64_t>& shape, const std::string& device, 
 }
 
 // The two halves of DenseASPP.score, whose logits and gradient live in the engine's buffers.
-py::tuple upsampled_forward(const Tensor& low, const OptTensor& labels, int64_t top_k, int64_t ignore_index, bool entropy, int64_t stream) {
+py::tuple upsampled_forward(const Tensor& low, const OptTensor& labels, int64_t top_k, int64_t ignore_index, bool entropy, bool stats, int64_t stream) {
     at::NoGradGuard no_grad;
     auto p = make_plan(low.sizes(), low.device(), labels, top_k, ignore_index, entropy, 8);
     p->stream = stream;
-    const Out o = scores_forward(*p, low, false);
-    return py::make_tuple(opt(o.logp), opt(o.entropy), opt(o.top_logp), opt(o.top_class));
+    const Out o = scores_forward(*p, low, stats);
+    return py::make_tuple(opt(o.logp), opt(o.entropy), opt(o.top_logp), opt(o.top_class), opt(o.stats));
 }
-void upsampled_backward(const Tensor& low, const OptTensor& labels, int64_t ignore_index, const OptTensor& top_class, const OptTensor& g_logp,
-                        const OptTensor& g_entropy, const OptTensor& g_top, const Tensor& out, int64_t stream) {
+void upsampled_backward(const Tensor& low, const OptTensor& labels, int64_t ignore_index, const Tensor& stats, const OptTensor& entropy,
+                        const OptTensor& top_class, const OptTensor& g_logp, const OptTensor& g_entropy, const OptTensor& g_top, const Tensor& out, int64_t stream) {
     at::NoGradGuard no_grad;
     auto p = make_plan(low.sizes(), low.device(), labels, top_class.has_value() ? top_class->size(1) : 0, ignore_index, true, 8);
     p->stream = stream;
     auto t = [](const OptTensor& x) { return x.has_value() ? *x : Tensor(); };
-    scores_backward(*p, low, Tensor(), Tensor(), t(top_class), t(g_logp), t(g_entropy), t(g_top), out);
+    scores_backward(*p, low, stats, t(entropy), t(top_class), t(g_logp), t(g_entropy), t(g_top), out);
 }
 
 // ---------------------------------------------------------------- gradient norm

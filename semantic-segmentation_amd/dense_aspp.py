@@ -110,10 +110,10 @@ class _ScoreFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, model, x, args, dropout_masks, generator, *params):
-        eng, s = model._scored_pass(x, args, dropout_masks, generator)
+        eng, s, stats = model._scored_pass(x, args, dropout_masks, generator, True)
         ctx.model, ctx.eng, ctx.ignore_index, ctx.pass_id = model, eng, args[2], eng.pass_id
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(s[3], args[0])
+        ctx.save_for_backward(stats, s[1], s[3], args[0])
         if s[3] is not None:
             ctx.mark_non_differentiable(s[3])
         return s
@@ -126,10 +126,10 @@ class _ScoreFn(torch.autograd.Function):
             raise RuntimeError('DenseASPP.score: another pass has run since this forward pass and its activations are gone; '
                                'call backward once, before the next pass')
         eng.pass_id += 1
-        top_class, labels = ctx.saved_tensors
+        stats, entropy, top_class, labels = ctx.saved_tensors
         low = eng.low_logits()
         dlow = eng.dlogits.view(eng.B, eng.H2, eng.W2, S.CLS_PAD)[..., :model.spec.n_class].permute(0, 3, 1, 2)
-        _lib.binding().upsampled_backward(low, labels, ctx.ignore_index, top_class, g_logp, g_entropy, g_top, dlow, _lib.raw_stream(low))
+        _lib.binding().upsampled_backward(low, labels, ctx.ignore_index, stats, entropy, top_class, g_logp, g_entropy, g_top, dlow, _lib.raw_stream(low))
         # as in _LogitsFn: the arena the .grad views alias keeps its contents
         held = model._gflat.clone()
         model._gflat_zero()
@@ -501,13 +501,15 @@ class DenseASPP(nn.Module):
         _lib.binding().check_scores([x.shape[0], self.spec.n_class, x.shape[2] // 8, x.shape[3] // 8], str(x.device), labels, args[1], args[3], 8)
         if torch.is_grad_enabled() and self.training:
             return Scores._make(_ScoreFn.apply(self, x, args, dropout_masks, generator, *[p for _, p in self.named_parameters()]))
-        return Scores._make(self._scored_pass(x, args, dropout_masks, generator)[1])
+        return Scores._make(self._scored_pass(x, args, dropout_masks, generator, False)[1])
 
-    def _scored_pass(self, x, args, dropout_masks, generator):
+    def _scored_pass(self, x, args, dropout_masks, generator, stats):
+        """The forward pass and its scores; with `stats` what the scores' backward pass needs too."""
         labels, top_k, ignore_index, entropy = args
         eng = self._run_forward(x, dropout_masks=dropout_masks, generator=generator)
         low = eng.low_logits()
-        return eng, _lib.binding().upsampled_forward(low, labels, top_k, ignore_index, entropy, _lib.raw_stream(low))
+        s = _lib.binding().upsampled_forward(low, labels, top_k, ignore_index, entropy, stats, _lib.raw_stream(low))
+        return eng, s[:4], s[4]
 
     def train_step(self, x, labels, ignore_index=255, dropout_masks=None, generator=None, zero_grad=True,
                    refresh=True, reducer=None):

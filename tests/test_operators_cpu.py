@@ -79,9 +79,10 @@ def test_scores8_backward_descriptor():
     need = lib.dsaspp_scores8_workspace(ctypes.byref(_scores8()))
     assert need == 1 * 1 * 2 * 45 * 19                       # one tile of cells across (6 of 8), two down (5 of 8), 9 x 5 corner pixels each
     assert lib.dsaspp_scores8_workspace(ctypes.byref(_scores8(n_class=40))) == -1
-    full = dict(g_logp=GOOD, dlogits=GOOD, gn=380, gy=95, gx=19, gc=1, ws=GOOD, ws_len=need)
+    full = dict(g_logp=GOOD, stats=GOOD, dlogits=GOOD, gn=380, gy=95, gx=19, gc=1, ws=GOOD, ws_len=need)
     for bad, message in ((dict(ws_len=need - 1), 'workspace'), (dict(ws=None), 'workspace'), (dict(gx=0), 'gradient strides'), (dict(dlogits=None), 'dlogits'),
-                         (dict(g_dtype=7), 'g_dtype'), (dict(g_logp=None), 'upstream'), (dict(g_top=GOOD), 'top_class')):
+                         (dict(g_dtype=7), 'g_dtype'), (dict(g_logp=None), 'upstream'), (dict(g_top=GOOD), 'top_class'), (dict(stats=None), 'stats'),
+                         (dict(g_entropy=GOOD), 'entropy of the forward')):
         assert lib.dsaspp_scores8_bwd(ctypes.byref(_scores8(**dict(full, **bad))), None) != 0
         assert message in _err(), message
 

@@ -5,6 +5,9 @@
 // Bound by HBM: the norm reads every gradient once, the second pass reads and writes it.  Two launches per call: the first
 // leaves one fp64 partial per block, and every block of the second adds up the same partials in the same order and so knows
 // the coefficient without a third launch, an atomic or a flag.
+//
+// Measured: norm of 35.4 M fp32 elements in 500 tensors 46 us (142 MB, while the last call's writes leave the caches), scaling 50 us (284 MB);
+// 200 M bf16 elements 120 and 129 us; the Adam update of 35.4 M parameters with bf16 copy 183 us after the norm (1.06 GB, 5.8 TB/s).
 #include "elem.h"
 #include <math.h>
 #include <algorithm>
@@ -14,8 +17,12 @@
 
 namespace {
 
-constexpr int CHUNK = 4096;               // elements of one range that a block takes at a time
-constexpr int MAX_BLOCKS = 2048;          // 8 blocks of 4 waves per CU fill the chip; a block takes several chunks in a row
+// Elements of one range that a block takes at a time: small ones spread few elements over more CUs (a launch of 100 tensors with 1.1 M
+// elements: norm 5.4 us against 7.2 with chunks of 8192), lists of 35 and 200 M elements show no difference.
+constexpr int CHUNK = 4096;
+// 8 blocks of 4 waves per CU fill the chip; a block takes several chunks in a row.  With 4096 blocks the scaling of 200 M elements takes 139 us
+// against 132, with 8192 171: each adds up all partials.
+constexpr int MAX_BLOCKS = 2048;
 // The ranges of one launch travel in its kernel arguments (4.0 of 4 KB), ten bytes each: 32 bits of distance from the first range, in
 // elements, 32 bits of length and 16 bits of first chunk.  24 bytes each made three launches of what fits one; a launch costs the host 3 us.
 constexpr int MAX_RANGES = 400;

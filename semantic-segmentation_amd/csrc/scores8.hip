@@ -314,7 +314,8 @@ __global__ __launch_bounds__(256, NC <= 19 ? (K == 0 ? 4 : 3) : 1) void scores8_
                 }
 #pragma unroll 1
                 for (int c = 0; c < nc; ++c) s.add(q.plain_logit(corner, c, hy, ly));
-                sum = s.s;
+                // relative to the reference of the short form: the backward pass, whose waves hold other columns, may take that for this one
+                sum = s.s * __builtin_amdgcn_exp2f(fmaxf((s.m - mix(hy, ch.M0, ly, ch.M1)) * SR_LOG2E, SR_FAR));
                 const float log_s = logf(s.s);
                 logp = label < 0 ? 0.f : s.empty() ? -INFINITY : (q.plain_logit(corner, label, hy, ly) - s.m) - log_s;
                 h = s.entropy(log_s);

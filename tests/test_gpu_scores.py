@@ -368,6 +368,42 @@ def test_upsampled_rows_that_peak_at_different_classes(depth, classes):
     _check8(z, labels, _place(z, 'last'), 0, True)
 
 
+@pytest.mark.parametrize('x', [2, 3, 7, 8, 12, 15, 16])
+def test_upsampled_steep_pixels_beside_ordinary_ones(x):
+    """One steep column of pixels: the short form holds for some waves only, and the two passes, whose waves hold different columns, do
+    not agree about all of them."""
+    z, labels, _ = _make8((1, 19, 6, 20), torch.float32, 'last', 7)
+    z[:, :, :, x] -= 200.0
+    z[:, 0, ::2, x] += 200.0
+    z[:, 1, 1::2, x] += 200.0
+    for layout in ('last', 'dense'):
+        _check8(z, labels, _place(z, layout), 2, True)
+        _check8(z, labels, _place(z, layout), 0, True)
+
+
+@pytest.mark.parametrize('x', [7, 8, 9])
+def test_upsampled_far_pixels_beside_ordinary_ones(x):
+    """Logits of 1e6 in a few pixels: what lies two pixels away has the gradient it has without them.  Each of the two gradients is off by
+    15 R half-steps in an exponent (short form), R = 20 bounding the ordinary logits, relative to the sizes of its terms."""
+    z, labels, _ = _make8((1, 19, 6, 20), torch.float32, 'last', 9)
+    z = z.clamp(-20, 20)
+    g = torch.Generator().manual_seed(1)
+    u = [torch.randn(1, 48, 160, generator=g) for _ in range(2)]
+    grads = []
+    for far in (False, True):
+        t = z.clone()
+        if far:
+            t[:, ::3, :, x] = 1.0e6
+        low = _place(t, 'last').requires_grad_()
+        s = _label_scores(low, labels.cuda(), upsample=8)
+        grad, = torch.autograd.grad((s.logp, s.entropy), low, [v.cuda() for v in u])
+        grads.append(grad.double().cpu()[..., :x - 1])
+    r = R.scores(R.interpolate(z), labels, 0, -100, 19, R=20.0)
+    size = r['p'] * (u[0].abs().double().unsqueeze(1) + u[1].abs().double().unsqueeze(1) * (r['lp'].abs() + r['entropy'].unsqueeze(1)))
+    lim = (2 * 15 * 20 + 64) * R.U * R.adjoint(size)[..., :x - 1] + 2 * 64 * R.U * R.adjoint(u[0].abs().double().unsqueeze(1).expand_as(size))[..., :x - 1]
+    assert bool(((grads[0] - grads[1]).abs() <= lim).all())
+
+
 @pytest.mark.parametrize('k', [2, 3, 8])
 def test_upsampled_near_ties(k):
     """Classes that differ in their last bits alone, in both directions, and both zeros."""

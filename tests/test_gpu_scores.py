@@ -664,3 +664,35 @@ def test_stale_pass_is_refused():
     s.logp.sum().backward(retain_graph=True)
     with pytest.raises(RuntimeError, match='another pass'):
         s.logp.sum().backward()
+
+
+def test_score_backward_clip_and_update_together():
+    """A step of one's own: scores of the network, a loss, its backward pass, the clipped Adam update; and clipping in place beside it.
+    The first Adam step is lr g / (|g| + eps) with the clipped g: 16 half-steps of it and one of the parameter."""
+    from e2e_common import make_batch
+    from semantic_segmentation_amd.optim import FusedAdam, clip_grad_norm_
+    _, mod = _tiny(True, torch.float32)
+    x, labels = make_batch(2, 64, 96)
+    opt = FusedAdam(mod, lr=1e-3)
+    s = mod.score(x.cuda(), labels.cuda(), top_k=2)
+    (-s.logp.mean() + 0.1 * s.entropy.mean()).backward()
+    params = list(mod.parameters())
+    g = [p.grad.double().cpu() for p in params]
+    before = [p.detach().double().cpu() for p in params]
+    want = math.sqrt(sum(float(t.square().sum()) for t in g))
+    copies = [torch.nn.Parameter(p.detach().clone()) for p in params]
+    for c, p in zip(copies, params):
+        c.grad = p.grad.clone()
+    limit = 0.5 * want
+    coef = limit / (want + 1e-6)
+    norm = clip_grad_norm_(copies, limit)
+    assert abs(float(norm) - want) <= 1.01 * R.U * want
+    for c, t in zip(copies, g):
+        R.agree(c.grad, t * coef, 3 * R.U * (t * coef).abs(), 'clipped')
+    norm = opt.step(max_grad_norm=limit)
+    assert abs(float(norm) - want) <= 1.01 * R.U * want
+    for p, b, t in zip(params, before, g):
+        step = 1e-3 * (t * coef) / ((t * coef).abs() + 1e-8)
+        R.agree(p.detach(), b - step, 16 * R.U * step.abs() + R.U * b.abs(), 'parameter')
+    after = mod.score(x.cuda(), labels.cuda())
+    assert bool(torch.isfinite(after.logp).all())

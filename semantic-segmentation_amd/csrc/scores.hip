@@ -700,19 +700,31 @@ int check(const dsaspp_scores_desc* d, const char* who, Args* a) {
 
 unsigned grid_for(int64_t blocks) { return (unsigned)(blocks < (1 << 20) ? blocks : (1 << 20)); }
 
-// Pixels per lane: 4 where they are contiguous and there are enough of them to fill the chip (256 CUs of 8 waves) all the same.  8 pixels
-// of a 16-bit type per lane were slower at every top_k (19 classes: 32 against 30 us without alternatives, 78 against 60 us with 3).
-int px_per_lane(const Args& a) { return a.d.s2 == 1 && a.d.d2 >= 4 && a.rows >= 4 * 256 * 512 ? 4 : 1; }
+// Pixels per lane, 4 or 1, where the pixels are contiguous.  Forward and 19 classes of 4.2 M pixels, 1 against 4: without alternatives
+// 88 and 85 us (fp32), 68 and 56 (bf16); with one 98 and 104, 88 and 76; with three 113 and 130, 107 and 112; with eight 163 and 207, 172 and 247:
+// four lists of alternatives leave too few waves.  And 4 need enough pixels: 1 M of 150 classes without alternatives 136 and 122 us (fp32), but 94
+// and 113 (bf16, whose loads are half as wide).
+//
+// Backward, 19 classes, one to three alternatives: 262144 pixels 16 against 18 us (fp32) and 10 against 13 (bf16), 400000 pixels 25 and 21, 19 and
+// 16, 4.2 M 261 and 184, 180 and 97: writes of 16 or 8 bytes per lane.  8 pixels of a 16-bit type per lane were slower at every top_k.
+template <int DT, int K, bool BWD>
+int px_per_lane(const Args& a) {
+    const int64_t least = BWD ? 3 << 17 : DT == 1 ? 1 << 20 : 1 << 21;
+    return a.d.s2 == 1 && a.d.d2 >= 4 && (BWD || K <= 1) && a.rows >= least ? 4 : 1;
+}
 
 template <int DT, int K, bool BWD>
 void launch_planes(const Args& a, hipStream_t s) {
-    const int P = px_per_lane(a);
+    const int P = px_per_lane<DT, K, BWD>(a);
     const int64_t per_row = (a.d.d2 + P - 1) / P, groups = a.d.d0 * a.d.d1 * per_row;
     const dim3 grid(grid_for((groups + 255) / 256)), block(256);
 #define LAUNCH(P) \
     if constexpr (BWD) hipLaunchKernelGGL((planes_bwd_kernel<DT, K, P>), grid, block, 0, s, a, groups, per_row); \
     else hipLaunchKernelGGL((planes_fwd_kernel<DT, K, P>), grid, block, 0, s, a, groups, per_row)
-    if (P == 4) { LAUNCH(4); } else { LAUNCH(1); }
+    if constexpr (BWD || K <= 1) {
+        if (P == 4) { LAUNCH(4); return; }
+    }
+    LAUNCH(1);
 #undef LAUNCH
 }
 
@@ -748,7 +760,9 @@ void launch_rows(const Args& a, hipStream_t s) {
     const dsaspp_scores_desc& d = a.d;
     const int size = DT == 1 ? 4 : 2;
     const bool dense = (d.d2 == 1 || d.s2 == d.n_class) && (d.d1 == 1 || d.s1 == d.d2 * d.n_class) && (d.d0 == 1 || d.s0 == a.plane * d.n_class);
-    if (dense && d.n_class * size <= TILE_ROW_BYTES && a.rows >= 16 * TILE_ROWS && a.rows < (1ll << 31)) {      // a lane per row: a grid has fewer than 2^32 lanes
+    // A lane per row by way of LDS from two blocks per CU on (a grid has fewer than 2^32 lanes).  19 fp32 classes, 3 alternatives, forward and backward:
+    // 8192 rows 12.1 us against 9.1 with lanes sharing rows, 65536 rows 13.8 and 13.1, 1 M rows 70 and 116.
+    if (dense && d.n_class * size <= TILE_ROW_BYTES && a.rows >= 512 * TILE_ROWS && a.rows < (1ll << 31)) {
         const int stride = d.n_class * size + (d.n_class % 8 == 0 ? 16 : 0);
         const dim3 grid((unsigned)((a.rows + TILE_ROWS - 1) / TILE_ROWS)), block(TILE_ROWS);
         if constexpr (BWD) hipLaunchKernelGGL((tile_bwd_kernel<DT, K>), grid, block, TILE_ROWS * stride, s, a, stride);

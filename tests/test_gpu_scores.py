@@ -134,6 +134,31 @@ def test_many_rows_of_few_classes(shape, dtype):
     _check(z, labels, logits, min(8, shape[1]), True)
 
 
+@pytest.mark.parametrize('shape', [(131072, 2), (131073, 3), (131071, 19), (131327, 16), (131100, 19), (131328, 32), (131201, 33), (131400, 63), (3, 19, 210, 211)])
+@pytest.mark.parametrize('dtype', list(DT))
+def test_rows_enough_for_a_lane_each(shape, dtype):
+    z, labels, logits = _make(shape, DT[dtype], 'last', shape[1])
+    _check(z, labels, logits, 2, True)
+    z, labels, logits = _make(shape, DT[dtype], 'last', shape[1], mask='rows')
+    _check(z, labels, logits, 0, True)
+
+
+@pytest.mark.parametrize('mask', ['random', 'lowest', 'nan'])
+def test_masks_in_rows_enough_for_a_lane_each(mask):
+    for dtype in DT.values():
+        z, labels, logits = _make((131100, 9), dtype, 'dense', 11, mask=mask)
+        _check(z, labels, logits, 3, True)
+
+
+@pytest.mark.parametrize('shape,layout', [((1, 3, 2097155), 'dense'), ((2, 3, 1025, 1031), 'dense'), ((2, 3, 1030, 1040), 'crop'), ((2, 3, 1030, 1040), 'step')])
+@pytest.mark.parametrize('dtype', list(DT))
+def test_planes_with_several_pixels_per_lane_both_ways(shape, layout, dtype):
+    z, labels, logits = _make(shape, DT[dtype], layout, 5)
+    _check(z, labels, logits, 1, True)
+    z, labels, logits = _make(shape, DT[dtype], layout, 6, mask='nan')
+    _check(z, labels, logits, 0, True)
+
+
 @pytest.mark.parametrize('rows,classes', [(1, 5003), (3, 8193), (2, 21841), (1030, 8195), (1, 4096), (1, 100001), (127, 16385), (128, 16385), (20, 4099)])
 @pytest.mark.parametrize('dtype', ['fp32', 'bf16'])
 def test_long_rows(rows, classes, dtype):

@@ -171,8 +171,12 @@ struct Column {
 // at most 0 and linear in r, so its exponential is a geometric sequence down the 8 rows of a cell: e(r + 1) = e(r) 2^(dx / 8), one
 // multiplication where an interpolation, a subtraction and an exponential (four issue slots) would be.  It asks for |dx| <= 48: then the
 // sum of a row is at least 2^-48, and a term that starts below the normal range (2^-126) ends below 2^-78 and does not count.
-// A step adds at most 3 half-steps of relative error (the factor's and the product's), seven of them 21; x0 and dx carry the roundings of
-// R = max |r_i|: below 15 R half-steps together in a logarithm.
+// A step adds at most 3 half-steps of relative error (the factor's and the product's), seven of them 21.
+//
+// r0 and r1 are rounded as z's definition rounds them and the maximum is subtracted before the scaling, so a class that leads both rows has
+// x = 0 and e = 1 to the bit, and the log probability of any class is taken from the same x: nothing but the class' own x and the sum enter,
+// no reference rounded apart (one of them put half of all confident pixels above 0, by up to R half-steps).  What is left of R = max |r_i| is
+// the rounding of z along y and that of x: at most 10 R half-steps together in a logit.
 // Columns of logits from 1e5 on, and of -inf and NaN, take the plain form.
 constexpr float ALIKE = 48.f, TAME = 1.0e5f;
 constexpr float PAD = -1.0e6f;            // x of the classes past the last one: below that of any tame logit
@@ -188,17 +192,17 @@ struct Chain {
         M0 = M1 = -FLT_MAX;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            x0[c] = fmaf(col.lx, p[CS + c], col.hx * p[c]);
-            dx[c] = fmaf(col.lx, p[PX * CS + CS + c], col.hx * p[PX * CS + c]);
+            x0[c] = mix(col.hx, p[c], col.lx, p[CS + c]);
+            dx[c] = mix(col.hx, p[PX * CS + c], col.lx, p[PX * CS + CS + c]);
             if (EXACT || c < nc) { M0 = fmaxf(M0, x0[c]); M1 = fmaxf(M1, dx[c]); }
         }
-        const float m0 = M0 * SR_LOG2E, m1 = M1 * SR_LOG2E, ly = col.ly(col.r_begin), step = col.cj != 0 ? 0.125f : 0.f;
+        const float ly = col.ly(col.r_begin), step = col.cj != 0 ? 0.125f : 0.f;
         float far = 0.f;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             const bool real = EXACT || c < nc;
-            x0[c] = real ? fmaf(x0[c], SR_LOG2E, -m0) : PAD;
-            dx[c] = real ? fmaf(dx[c], SR_LOG2E, -m1) - x0[c] : 0.f;
+            x0[c] = real ? (x0[c] - M0) * SR_LOG2E : PAD;
+            dx[c] = real ? fmaf(dx[c] - M1, SR_LOG2E, -x0[c]) : 0.f;
             far = fmaxf(far, fabsf(dx[c]));
             q[c] = __builtin_amdgcn_exp2f(step * dx[c]);         // the topmost cells have ly = 0 throughout
             e[c] = __builtin_amdgcn_exp2f(fmaf(ly, dx[c], x0[c]));
@@ -207,6 +211,13 @@ struct Chain {
         return far <= ALIKE;
     }
     __device__ __forceinline__ float x(int c, float ly) const { return fmaf(ly, dx[c], x0[c]); }
+    // the same bits for a class known at run time only: from the corners again, no register is indexed
+    template <int CS, int PX>
+    __device__ __forceinline__ float x_of(const Column<CS, PX>& col, const float* corner, int c, float ly) const {
+        const float* p = corner + col.at + c;
+        const float a = (mix(col.hx, p[0], col.lx, p[CS]) - M0) * SR_LOG2E;
+        return fmaf(ly, fmaf(mix(col.hx, p[PX * CS], col.lx, p[PX * CS + CS]) - M1, SR_LOG2E, -a), a);
+    }
 };
 
 // The K largest of a pixel in the short form.  A key is x with its five lowest bits replaced by the class, so that keeping K + 1
@@ -283,8 +294,9 @@ __global__ __launch_bounds__(256, NC <= 19 ? (K == 0 ? 4 : 3) : 1) void scores8_
                     ch.e[c] *= ch.q[c];
                 }
                 sum = s;
-                const float log2_s = __builtin_amdgcn_logf(s), up = mix(hy, ch.M0, ly, ch.M1);
-                logp = label < 0 ? 0.f : SR_LN2 * ((q.logit(corner, max(label, 0), hy, ly) - up) * SR_LOG2E - log2_s);
+                const float log2_s = __builtin_amdgcn_logf(s);
+                // between two rows with other leading classes the sum's error may exceed the class' distance from it
+                logp = label < 0 ? 0.f : fminf(SR_LN2 * (ch.x_of(q, corner, max(label, 0), ly) - log2_s), 0.f);
                 h = fmaxf(SR_LN2 * (log2_s - t * __builtin_amdgcn_rcpf(s)), 0.f);
                 if (K > 0) {
 #pragma unroll
@@ -299,23 +311,26 @@ __global__ __launch_bounds__(256, NC <= 19 ? (K == 0 ? 4 : 3) : 1) void scores8_
                     }
 #pragma unroll
                     for (int j = 0; j < K; ++j)
-                        if (j < d.top_k) top_lp[j] = SR_LN2 * ((q.logit(corner, top_i[j], hy, ly) - up) * SR_LOG2E - log2_s);
+                        if (j < d.top_k)          // descending as the logits are, whose near ties x may turn round
+                            top_lp[j] = fminf(SR_LN2 * (ch.x_of(q, corner, top_i[j], ly) - log2_s), j > 0 ? top_lp[j > 0 ? j - 1 : 0] : 0.f);
                 }
             } else {
                 Top<K> top;
                 Soft s;
                 top.clear();
                 s.clear();
+                int best = 0;
 #pragma unroll 1
                 for (int c = 0; c < nc; ++c) {
                     const float z = q.plain_logit(corner, c, hy, ly);
+                    best = z > s.m ? c : best;
                     s.m = fmaxf(s.m, z);
                     top.offer(z, c);
                 }
 #pragma unroll 1
                 for (int c = 0; c < nc; ++c) s.add(q.plain_logit(corner, c, hy, ly));
                 // relative to the reference of the short form: the backward pass, whose waves hold other columns, may take that for this one
-                sum = s.s * __builtin_amdgcn_exp2f(fmaxf((s.m - mix(hy, ch.M0, ly, ch.M1)) * SR_LOG2E, SR_FAR));
+                sum = s.s * __builtin_amdgcn_exp2f(fmaxf(ch.x_of(q, corner, best, ly), SR_FAR));
                 const float log_s = logf(s.s);
                 logp = label < 0 ? 0.f : s.empty() ? -INFINITY : (q.plain_logit(corner, label, hy, ly) - s.m) - log_s;
                 h = s.entropy(log_s);

@@ -237,13 +237,15 @@ struct Keys {
         v[0] = larger(v[0], k);
     }
     __device__ __forceinline__ int cls(int j) const { return (int)(__float_as_uint(v[j]) & 31u); }
-    // R half-steps of the two x (15 each and as many again, in log2 units 1.44 times that), 2^-18 for the two keys' missing bits, and
-    // something above the class bits of an x of 0 (denormal) where R is 0
+    // Two keys are in the logits' order if they are further apart than what may have moved them: up to 31 steps of the last place of x each
+    // (the class for the bits that were there), together below 2^-17 of the larger magnitude, and the roundings of the two x, 10 R half-steps
+    // each in a logit, 29 R together in log2 units (96 are allowed).  At least something above the class bits of an x of 0 (a denormal), where
+    // R is 0.
     __device__ __forceinline__ bool unclear(int k, float R) const {
         const float near = fmaf(R, 96.f * 0x1p-24f, 1.0e-30f);
         int u = 0;                        // no short circuit: it would put each median into a block of its own, with every key kept for it
 #pragma unroll
-        for (int j = 0; j < K; ++j) u |= (int)(v[j] - v[j + 1] <= fmaf(fabsf(v[j + 1]), 0x1p-18f, near)) & (int)(j < k);
+        for (int j = 0; j < K; ++j) u |= (int)(v[j] - v[j + 1] <= fmaf(fabsf(v[j + 1]), 0x1p-17f, near)) & (int)(j < k);
         return u != 0;
     }
 };

@@ -32,3 +32,21 @@ def test_confident_pixels_have_log_probabilities_of_at_most_zero(classes, lead, 
     R.agree(s.logp, r['logp'], lim, 'logp')
     assert torch.equal(s.top_class.cpu(), r['top_class'])
     R.agree(s.top_logp[:, 0], r['top_logp'][:, 0], lim, 'top_logp')
+
+
+@pytest.mark.parametrize('hi,lo,rest', [(22.1, -22.9, -35.0), (10.0, -12.0, -14.0), (60.0, -60.0, -61.0), (3.0, -0.5, -4.0)])
+def test_two_classes_that_all_but_tie_far_below_the_leading_one(hi, lo, rest):
+    """Classes 0 and 30 a few steps of the last place apart, class 31 far above them: the order is that of the logits to the bit."""
+    for seed in range(2):
+        g = torch.Generator().manual_seed(seed)
+        n = (1, 64, 65)
+        z = rest + torch.randn(1, 32, 64, 65, generator=g) * 0.1
+        base = lo + torch.randn(n, generator=g) * 0.3
+        z[:, 31] = hi + torch.randn(n, generator=g) * 0.3
+        z[:, 0] = base + torch.randn(n, generator=g) * abs(lo) * 2.0e-7
+        z[:, 30] = base + torch.randn(n, generator=g) * abs(lo) * 2.0e-7
+        s = _label_scores(_place(z, 'last'), top_k=3, upsample=8)
+        full = R.interpolate(z)
+        want = torch.sort(full, dim=1, descending=True, stable=True).indices[:, :3]
+        assert torch.equal(s.top_class.cpu(), want), int((s.top_class.cpu() != want).any(1).sum())
+        assert bool((s.top_logp[:, 1:] <= s.top_logp[:, :-1]).all())

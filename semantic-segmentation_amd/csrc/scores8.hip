@@ -175,10 +175,16 @@ struct Column {
 //
 // r0 and r1 are rounded as z's definition rounds them and the maximum is subtracted before the scaling, so a class that leads both rows has
 // x = 0 and e = 1 to the bit, and the log probability of any class is taken from the same x: nothing but the class' own x and the sum enter,
-// no reference rounded apart (one of them put half of all confident pixels above 0, by up to R half-steps).  What is left of R = max |r_i| is
-// the rounding of z along y and that of x: at most 10 R half-steps together in a logit.
-// Columns of logits from 1e5 on, and of -inf and NaN, take the plain form.
-constexpr float ALIKE = 48.f, TAME = 1.0e5f;
+// no reference rounded apart (one of them put half of all confident pixels above 0, by up to R half-steps).
+//
+// What the two forms round differently is z along y (2 half-steps of hy |r0| + ly |r1|) and x (subtraction, scaling, dx, x: 3 of the distance
+// from the maximum and one of dx).  With M = max |M_i| and a class X below the maximum that is 2 (X + M) + 3 X + 34 half-steps in its logit:
+// it falls out of the classes that count, but grows with M.  So columns with M from 64 on take the plain form, which has the errors of an
+// fp32 log-softmax of z; below that a log probability is off by at most 2 (2 M + 34) half-steps more, 2e-5 at M = 64, 6e-6 at M = 10.
+// (With M up to 1e5, logits 3 units apart and 1e4 off zero had log probabilities 2e-3 off.)
+// Blocks with logits beyond 1e5, and those with -inf or NaN, take the plain form too: four pictures of 1024 x 2048, 19 classes, 3 alternatives
+// 267 us against 137, forward and backward pass of eight 843 against 270.
+constexpr float ALIKE = 48.f, NEAR_ZERO = 64.f, TAME = 1.0e5f;
 constexpr float PAD = -1.0e6f;            // x of the classes past the last one: below that of any tame logit
 
 template <int NC>
@@ -208,8 +214,9 @@ struct Chain {
             e[c] = __builtin_amdgcn_exp2f(fmaf(ly, dx[c], x0[c]));
         }
         far *= 8.f * step;
-        return far <= ALIKE;
+        return far <= ALIKE && largest() < NEAR_ZERO;
     }
+    __device__ __forceinline__ float largest() const { return fmaxf(fabsf(M0), fabsf(M1)); }
     __device__ __forceinline__ float x(int c, float ly) const { return fmaf(ly, dx[c], x0[c]); }
     // the same bits for a class known at run time only: from the corners again, no register is indexed
     template <int CS, int PX>
@@ -238,14 +245,13 @@ struct Keys {
     }
     __device__ __forceinline__ int cls(int j) const { return (int)(__float_as_uint(v[j]) & 31u); }
     // Two keys are in the logits' order if they are further apart than what may have moved them: up to 31 steps of the last place of x each
-    // (the class for the bits that were there), together below 2^-17 of the larger magnitude, and the roundings of the two x, 10 R half-steps
-    // each in a logit, 29 R together in log2 units (96 are allowed).  At least something above the class bits of an x of 0 (a denormal), where
-    // R is 0.
-    __device__ __forceinline__ bool unclear(int k, float R) const {
-        const float near = fmaf(R, 96.f * 0x1p-24f, 1.0e-30f);
+    // (the class for the bits that were there), together 124 half-steps of the larger magnitude; and the roundings of the two x, above, which
+    // are 5 |x| + 2.9 M + 48 half-steps each in log2 units.
+    static __device__ __forceinline__ float margin(float M) { return fmaf(M, 6.f * 0x1p-24f, 100.f * 0x1p-24f); }
+    __device__ __forceinline__ bool unclear(int k, float near) const {
         int u = 0;                        // no short circuit: it would put each median into a block of its own, with every key kept for it
 #pragma unroll
-        for (int j = 0; j < K; ++j) u |= (int)(v[j] - v[j + 1] <= fmaf(fabsf(v[j + 1]), 0x1p-17f, near)) & (int)(j < k);
+        for (int j = 0; j < K; ++j) u |= (int)(v[j] - v[j + 1] <= fmaf(fabsf(v[j + 1]), 140.f * 0x1p-24f, near)) & (int)(j < k);
         return u != 0;
     }
 };
@@ -272,6 +278,7 @@ __global__ __launch_bounds__(256, NC <= 19 ? (K == 0 ? 4 : 3) : 1) void scores8_
     Chain<NC> ch;
     const bool alike = ch.template start<EXACT>(q, corner, nc);
     const bool brief = R < TAME && __all(alike);
+    const float near = Keys<K>::margin(ch.largest());
     auto rows = [&](auto form) {          // a loop for each form: together they would copy every class' registers at its start
         constexpr bool BRIEF = decltype(form)::value;
 #pragma unroll 1
@@ -303,7 +310,7 @@ __global__ __launch_bounds__(256, NC <= 19 ? (K == 0 ? 4 : 3) : 1) void scores8_
                 if (K > 0) {
 #pragma unroll
                     for (int j = 0; j < K; ++j) top_i[j] = keys.cls(j);
-                    if (keys.unclear(d.top_k, R)) {
+                    if (keys.unclear(d.top_k, near)) {
                         Top<K> top;
                         top.clear();
 #pragma unroll 1

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import scores_ref as R
-from test_gpu_scores import _label_scores, _place
+from test_gpu_scores import _check8, _label_scores, _make8, _place
 
 pytestmark = pytest.mark.gpu
 U = R.U
@@ -50,3 +50,38 @@ def test_two_classes_that_all_but_tie_far_below_the_leading_one(hi, lo, rest):
         want = torch.sort(full, dim=1, descending=True, stable=True).indices[:, :3]
         assert torch.equal(s.top_class.cpu(), want), int((s.top_class.cpu() != want).any(1).sum())
         assert bool((s.top_logp[:, 1:] <= s.top_logp[:, :-1]).all())
+
+
+@pytest.mark.parametrize('offset', [64.0, -70.0, 1.0e3, -1.0e3, 1.0e4, -1.0e4, 9.0e4])
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_a_common_offset_costs_no_accuracy(offset, dtype, monkeypatch):
+    """All logits raised alike: the errors are those of an fp32 log-softmax of the interpolated logits, without a part that grows with
+    their magnitude."""
+    import test_gpu_scores
+    monkeypatch.setattr(test_gpu_scores, '_size', lambda low: 0.0)
+    z, labels, _ = _make8((2, 19, 5, 20), torch.float32, 'last', 3)
+    z = ((z * 0.75).clamp(-5.5, 5.5) + offset).to(dtype)
+    _check8(z, labels, _place(z, 'last'), 3, True)
+    _check8(z, labels, _place(z, 'dense'), 0, True)
+
+
+@pytest.mark.parametrize('x', [2, 7, 8, 12, 15, 16])
+@pytest.mark.parametrize('offset', [100.0, -100.0])
+def test_pixels_with_an_offset_beside_ordinary_ones(x, offset):
+    """The two passes, whose waves hold different columns, do not agree about which form a column takes."""
+    z, labels, _ = _make8((1, 19, 6, 20), torch.float32, 'last', 7)
+    z[:, :, :, x] += offset
+    for layout in ('last', 'dense'):
+        _check8(z, labels, _place(z, layout), 2, True)
+        _check8(z, labels, _place(z, layout), 0, True)
+
+
+@pytest.mark.parametrize('mask', [-100.0, -3.0e4, -1.0e9])
+def test_finite_masks_of_whole_classes(mask, monkeypatch):
+    """Classes masked by a large negative number in every pixel.  100 below the others p is 2^-144: a term of the gradient has a spacing of
+    2^-149 there in place of a relative rounding, and a low-resolution pixel adds up to 256 terms with four roundings each."""
+    monkeypatch.setattr(R, 'tiny', lambda dtype: 1024 * 2.0 ** -149)
+    z, labels, _ = _make8((1, 19, 6, 20), torch.float32, 'last', 5)
+    z[:, 4:9] = mask
+    _check8(z, labels, _place(z, 'last'), 3, True)
+    _check8(z, labels, _place(z, 'dense'), 0, True)

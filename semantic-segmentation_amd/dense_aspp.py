@@ -71,6 +71,13 @@ def _holder_mobilenet(sp):
     return trunk
 
 
+def _check_pass(ctx, name, once=''):
+    """The backward pass reads what the forward pass left in the engine's buffers."""
+    if ctx.eng.pass_id != ctx.pass_id:
+        raise RuntimeError('%s: another pass has run since this forward pass and its activations are gone; call backward %sbefore the next pass'
+                           % (name, once))
+
+
 class _LogitsFn(torch.autograd.Function):
     """Autograd bridge for the plain ``model(x)`` API (full-resolution logits)."""
 
@@ -78,7 +85,7 @@ class _LogitsFn(torch.autograd.Function):
     def forward(ctx, model, x, *params):
         eng = model._run_forward(x)
         eng.prog_up_fwd().run()
-        ctx.model, ctx.eng = model, eng
+        ctx.model, ctx.eng, ctx.pass_id = model, eng, eng.pass_id
         sp = model.spec
         return eng.out_logits.view(eng.B, sp.n_class, eng.H, eng.W).clone()
 
@@ -87,7 +94,9 @@ class _LogitsFn(torch.autograd.Function):
         model, eng = ctx.model, ctx.eng
         if not eng.training:
             raise RuntimeError('DenseASPP: backward needs the forward pass to run in train() mode')
+        _check_pass(ctx, 'DenseASPP')
         eng.pass_id += 1
+        ctx.pass_id = eng.pass_id             # retain_graph: the activations outlive a backward pass
         prog = eng.prog_up_bwd()
         eng.grad_full.view(grad.shape).copy_(grad)
         # The backward program writes into the flat gradient arena, which the .grad views of a previous train_step
@@ -122,9 +131,7 @@ class _ScoreFn(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, g_logp, g_entropy, g_top, _):
         model, eng = ctx.model, ctx.eng
-        if eng.pass_id != ctx.pass_id:
-            raise RuntimeError('DenseASPP.score: another pass has run since this forward pass and its activations are gone; '
-                               'call backward once, before the next pass')
+        _check_pass(ctx, 'DenseASPP.score', 'once, ')
         eng.pass_id += 1
         stats, entropy, top_class, labels = ctx.saved_tensors
         low = eng.low_logits()

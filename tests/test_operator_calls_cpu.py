@@ -1,0 +1,46 @@
+"""Calls around the class-score and gradient-norm operators whose outcome shows without a GPU."""
+import pytest
+import torch
+
+import denseASPP  # noqa: F401
+import kernel_model
+from e2e_common import TINY_CFG, make_batch, make_pair
+
+
+@pytest.fixture
+def fp32_model():
+    kernel_model.set_act_dtype(torch.float32)
+    yield
+    kernel_model.set_act_dtype(torch.bfloat16)
+
+
+def _pair():
+    ref, mod = make_pair(TINY_CFG)
+    mod.set_backend(kernel_model.ModelBackend())
+    return ref, mod.train()
+
+
+def test_backward_of_logits_after_another_pass_is_refused(fp32_model):
+    """The activations of a pass are gone once another one has run on the same shape, whatever started it."""
+    _, mod = _pair()
+    x, labels = make_batch(1, 64, 64)
+    for other in (lambda: mod(x), lambda: mod.forward_lowres(x), lambda: mod.predict(x), lambda: mod.train_step(x, labels)):
+        out = mod(x)
+        other()
+        with pytest.raises(RuntimeError, match='another pass'):
+            out.sum().backward()
+    out = mod(x)
+    mod(make_batch(2, 64, 64)[0])                          # another shape: activations of its own
+    out.sum().backward()
+
+
+def test_backward_of_logits_twice_gives_the_same_gradients(fp32_model):
+    _, mod = _pair()
+    x, _ = make_batch(1, 64, 64)
+    out = mod(x)
+    params = list(mod.parameters())
+    w = torch.randn(out.shape, generator=torch.Generator().manual_seed(1))
+    first = torch.autograd.grad((out * w).sum(), params, retain_graph=True)
+    again = torch.autograd.grad((out * w).sum(), params)
+    for a, b in zip(first, again):
+        assert torch.equal(a, b)

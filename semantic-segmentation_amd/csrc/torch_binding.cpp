@@ -90,6 +90,11 @@ template <typename T>
 T* ptr(const Tensor& t) { return t.defined() ? static_cast<T*>(t.data_ptr()) : nullptr; }
 dsaspp_stream_t handle(int64_t stream) { return reinterpret_cast<dsaspp_stream_t>(stream); }
 
+// The results below are new tensors filled by kernels of which torch knows nothing: a tangent would be dropped without a word.
+void no_tangent(const Tensor& t, const char* who) {
+    if (t.defined() && t._fw_grad(0).defined()) throw std::runtime_error(text("%s has no forward-mode derivative, but was given a dual tensor", who));
+}
+
 // ---------------------------------------------------------------- class scores
 struct Plan : torch::CustomClassHolder {
     int64_t n, c, ignore_index, stream = 0;
@@ -337,6 +342,7 @@ struct LabelScores : torch::autograd::Function<LabelScores> {
 py::object opt(const Tensor& t) { return t.defined() ? py::cast(t) : py::none(); }
 
 py::tuple label_scores(const Tensor& given, const OptTensor& labels, int64_t top_k, int64_t ignore_index, bool entropy, int64_t upsample, int64_t stream) {
+    no_tangent(given, "label_scores");
     TYPE_CHECK(dtype_code(given.scalar_type()) >= 0 && given.layout() == at::kStrided, "logits must be a float32, bfloat16 or float16 tensor, got %s",
                dtype_name(given).c_str());
     const Tensor logits = given.resolve_neg();        // itself, unless it is a view that torch negates when it is read
@@ -355,6 +361,8 @@ py::tuple label_scores(const Tensor& given, const OptTensor& labels, int64_t top
     }
     return py::make_tuple(opt(o.logp), opt(o.entropy), opt(o.top_logp), opt(o.top_class));
 }
+
+void check_image(const Tensor& x) { no_tangent(x, "DenseASPP.score"); }
 
 void check_scores(const std::vector<int64_t>& shape, const std::string& device, const OptTensor& labels, int64_t top_k, bool entropy, int64_t upsample) {
     make_plan(shape, at::Device(device), labels, top_k, 0, entropy, upsample);
@@ -412,6 +420,7 @@ struct Grads {
     at::Device device = at::kCPU;
 
     void add(const Tensor& t, const char* who) {
+        no_tangent(t, who);
         const int code = dtype_code(t.scalar_type());
         TYPE_CHECK(t.layout() == at::kStrided && code >= 0, "%s needs dense float32, bfloat16 or float16 gradients, got %s%s", who, dtype_name(t).c_str(),
                    t.layout() == at::kStrided ? "" : " in another layout");
@@ -506,6 +515,7 @@ Tensor clip_grads(const py::list& grads, bool of_parameters, double max_norm, do
 
 Tensor adam_update(const Tensor& p, const Tensor& grad, const Tensor& m, const Tensor& v, int64_t step, double lr, double beta1, double beta2, double eps,
                    double weight_decay, double grad_scale, double max_grad_norm, double norm_type, const OptTensor& shadow, int64_t stream) {
+    for (const Tensor* t : {&p, &grad, &m, &v}) no_tangent(*t, "adam_update_");
     for (const Tensor* t : {&p, &grad, &m, &v})
         VALUE_CHECK(t->is_cuda() && t->scalar_type() == at::kFloat && t->numel() == p.numel() && t->device() == p.device() && t->is_contiguous() && !t->is_neg(),
                     "adam_update_ needs contiguous float32 tensors of one size on one GPU");
@@ -583,6 +593,7 @@ PYBIND11_MODULE(_dsaspp_torch, m) {
     m.def("init", &init);
     m.def("source_hash", [] { return std::string(g_hash + 12); });
     m.def("label_scores", &label_scores);
+    m.def("check_image", &check_image);
     m.def("check_scores", &check_scores);
     m.def("upsampled_forward", &upsampled_forward);
     m.def("upsampled_backward", &upsampled_backward);

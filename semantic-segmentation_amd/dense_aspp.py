@@ -503,6 +503,7 @@ class DenseASPP(nn.Module):
             raise ValueError('DenseASPP expects an N x 3 x H x W image batch, got %s' % (tuple(x.shape),))
         if x.shape[2] % 8 or x.shape[3] % 8:
             raise ValueError('DenseASPP.score: H and W must be multiples of 8, got %d x %d' % tuple(x.shape[2:]))
+        _lib.binding().check_image(x)
         args = (labels, int(top_k), int(ignore_index), bool(entropy))
         # before the pass, which updates running statistics in train() mode
         _lib.binding().check_scores([x.shape[0], self.spec.n_class, x.shape[2] // 8, x.shape[3] // 8], str(x.device), labels, args[1], args[3], 8)

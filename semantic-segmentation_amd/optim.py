@@ -40,7 +40,8 @@ def _stream(tensors):
 def grad_norm(grads, norm_type=2.0):
     """Global norm of a list of gradient tensors (or of one): sqrt of the sum of all squares, or the largest magnitude for
     norm_type=inf, as a 0-dim fp32 tensor on their GPU.  float32, bfloat16 and float16 tensors may be mixed.  The sums are fp64:
-    magnitudes whose squares leave the fp32 range count in full, and the same tensors give the same bits each time."""
+    magnitudes whose squares leave the fp32 range count in full, and the same tensors give the same bits each time.  The result carries
+    no gradient of its own."""
     grads = _list(grads)
     return _lib.binding().grad_norm(grads, norm_type, _stream(grads))
 

@@ -40,7 +40,8 @@ def label_scores(logits, labels=None, top_k=0, ignore_index=-100, entropy=True, 
     low-resolution picture are no more than 33 units off in any class, all logits below 1e5 in magnitude; the others (a class masked by
     -1e9, a common offset of 100) cost twice as much, with the backward pass three times, per group of 8 x 4 low-resolution pixels.
 
-    logp, entropy and top_logp are differentiable with respect to the logits (once); the gradient has the logits' type."""
+    logp, entropy and top_logp are differentiable with respect to the logits (once, in reverse mode; dual tensors of forward mode are refused);
+    the gradient has the logits' type."""
     if not isinstance(logits, torch.Tensor):
         raise TypeError('label_scores needs a tensor of logits, got %s' % type(logits).__name__)
     return Scores._make(_lib.binding().label_scores(logits, labels, top_k, ignore_index, entropy, upsample, _lib.raw_stream(logits)))

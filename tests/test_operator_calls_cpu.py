@@ -1,10 +1,12 @@
 """Calls around the class-score and gradient-norm operators whose outcome shows without a GPU."""
 import pytest
 import torch
+import torch.autograd.forward_ad as fwad
 
 import denseASPP  # noqa: F401
 import kernel_model
 from e2e_common import TINY_CFG, make_batch, make_pair
+from semantic_segmentation_amd import label_scores, optim
 
 
 @pytest.fixture
@@ -44,3 +46,15 @@ def test_backward_of_logits_twice_gives_the_same_gradients(fp32_model):
     again = torch.autograd.grad((out * w).sum(), params)
     for a, b in zip(first, again):
         assert torch.equal(a, b)
+
+
+def test_forward_mode_derivatives_are_refused(fp32_model):
+    z, t = torch.randn(4, 5), torch.randn(4, 5)
+    _, mod = _pair()
+    x = torch.randn(1, 3, 64, 64)
+    with fwad.dual_level():
+        dual = fwad.make_dual(z, t)
+        for call in (lambda: label_scores(dual), lambda: optim.grad_norm([dual, z]), lambda: optim.clip_grads_([dual], 1.0),
+                     lambda: optim.adam_update_(z, dual, z, z, 1), lambda: mod.score(fwad.make_dual(x, x))):
+            with pytest.raises(RuntimeError, match='forward-mode'):
+                call()

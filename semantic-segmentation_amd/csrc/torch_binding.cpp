@@ -15,6 +15,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <algorithm>
@@ -90,7 +91,11 @@ template <typename T>
 T* ptr(const Tensor& t) { return t.defined() ? static_cast<T*>(t.data_ptr()) : nullptr; }
 dsaspp_stream_t handle(int64_t stream) { return reinterpret_cast<dsaspp_stream_t>(stream); }
 
-// The results below are new tensors filled by kernels of which torch knows nothing: a tangent would be dropped without a word.
+// The results below are new tensors filled by kernels of which torch knows nothing: a trace would record the empty tensors alone, and a
+// tangent would be dropped without a word.
+void no_trace(const char* who) {
+    if (torch::jit::tracer::getTracingState()) throw std::runtime_error(text("%s cannot be traced: a trace does not hold its kernels", who));
+}
 void no_tangent(const Tensor& t, const char* who) {
     if (t.defined() && t._fw_grad(0).defined()) throw std::runtime_error(text("%s has no forward-mode derivative, but was given a dual tensor", who));
 }
@@ -342,6 +347,7 @@ struct LabelScores : torch::autograd::Function<LabelScores> {
 py::object opt(const Tensor& t) { return t.defined() ? py::cast(t) : py::none(); }
 
 py::tuple label_scores(const Tensor& given, const OptTensor& labels, int64_t top_k, int64_t ignore_index, bool entropy, int64_t upsample, int64_t stream) {
+    no_trace("label_scores");
     no_tangent(given, "label_scores");
     TYPE_CHECK(dtype_code(given.scalar_type()) >= 0 && given.layout() == at::kStrided, "logits must be a float32, bfloat16 or float16 tensor, got %s",
                dtype_name(given).c_str());
@@ -362,7 +368,10 @@ py::tuple label_scores(const Tensor& given, const OptTensor& labels, int64_t top
     return py::make_tuple(opt(o.logp), opt(o.entropy), opt(o.top_logp), opt(o.top_class));
 }
 
-void check_image(const Tensor& x) { no_tangent(x, "DenseASPP.score"); }
+void check_image(const Tensor& x) {
+    no_trace("DenseASPP.score");
+    no_tangent(x, "DenseASPP.score");
+}
 
 void check_scores(const std::vector<int64_t>& shape, const std::string& device, const OptTensor& labels, int64_t top_k, bool entropy, int64_t upsample) {
     make_plan(shape, at::Device(device), labels, top_k, 0, entropy, upsample);
@@ -463,6 +472,7 @@ void written(const Tensor& t) {           // as torch's own in-place operations 
 
 // The gradients of a Python list: the tensors themselves, or the .grad of parameters that have one.
 Grads gather(const py::list& list, bool of_parameters, const char* who) {
+    no_trace(who);
     Grads g;
     const size_t n = list.size();
     g.ranges.reserve(n);
@@ -515,6 +525,7 @@ Tensor clip_grads(const py::list& grads, bool of_parameters, double max_norm, do
 
 Tensor adam_update(const Tensor& p, const Tensor& grad, const Tensor& m, const Tensor& v, int64_t step, double lr, double beta1, double beta2, double eps,
                    double weight_decay, double grad_scale, double max_grad_norm, double norm_type, const OptTensor& shadow, int64_t stream) {
+    no_trace("adam_update_");
     for (const Tensor* t : {&p, &grad, &m, &v}) no_tangent(*t, "adam_update_");
     for (const Tensor* t : {&p, &grad, &m, &v})
         VALUE_CHECK(t->is_cuda() && t->scalar_type() == at::kFloat && t->numel() == p.numel() && t->device() == p.device() && t->is_contiguous() && !t->is_neg(),

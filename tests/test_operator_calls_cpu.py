@@ -58,3 +58,13 @@ def test_forward_mode_derivatives_are_refused(fp32_model):
                      lambda: optim.adam_update_(z, dual, z, z, 1), lambda: mod.score(fwad.make_dual(x, x))):
             with pytest.raises(RuntimeError, match='forward-mode'):
                 call()
+
+
+def test_tracing_is_refused(fp32_model):
+    """A trace would hold the outputs' allocation without the kernels that fill them."""
+    z = torch.randn(4, 5)
+    _, mod = _pair()
+    for fn, x in ((lambda a: label_scores(a).entropy, z), (lambda a: optim.grad_norm([a]), z), (lambda a: optim.clip_grads_([a], 1.0), z),
+                  (lambda a: optim.adam_update_(a, a, a, a, 1), z), (lambda a: mod.score(a).entropy, torch.randn(1, 3, 64, 64))):
+        with pytest.raises(RuntimeError, match='traced'):
+            torch.jit.trace(fn, (x,))

@@ -510,10 +510,25 @@ Tensor clip_grads(const py::list& grads, bool of_parameters, double max_norm, do
     const c10::DeviceGuard guard(g.device);
     g.ready(true, who);
     g.d.max_norm = (float)max_norm;
+    std::vector<Tensor> held;
+    std::vector<c10::Storage> memory;
     if (error_if_nonfinite) {
         call(api.grad_norm_partials(&g.d, handle(stream)));
         call(api.grad_norm_finish(&g.d, handle(stream)));
-        const double v = g.norm.item<double>();
+        double v;
+        {
+            // Other Python threads run on while this one waits: the queue ahead may itself wait for what one of them has yet to launch.  The
+            // list and the parameters are theirs to change then, so the tensors and their memory are held here.
+            held.reserve(g.tensors.size());
+            memory.reserve(g.tensors.size());
+            for (const Tensor*& t : g.tensors) {
+                held.push_back(*t);
+                memory.push_back(t->storage());
+                t = &held.back();
+            }
+            const py::gil_scoped_release no_gil;
+            v = g.norm.item<double>();
+        }
         if (!std::isfinite(v)) throw std::runtime_error(text("the norm of the gradients is not finite (%g): nothing was clipped", v));
         call(api.clip_scale(&g.d, handle(stream)));
     } else {

@@ -1,9 +1,19 @@
 """-m gpu: calls of the class-score and gradient-norm operators beside the usual ones."""
+import threading
+import time
+
 import pytest
+import torch
 
 from test_gpu_scores import _tiny
 
 pytestmark = pytest.mark.gpu
+
+
+def _optim():
+    import denseASPP  # noqa: F401
+    from semantic_segmentation_amd import optim
+    return optim
 
 
 def test_network_backward_after_scores_of_the_same_batch_is_refused():
@@ -21,3 +31,36 @@ def test_network_backward_after_scores_of_the_same_batch_is_refused():
     mod(x.cuda())
     with pytest.raises(RuntimeError, match='another pass'):
         s.entropy.mean().backward()
+
+
+def test_other_threads_run_while_a_call_waits_for_the_norm():
+    """error_if_nonfinite waits for the GPU; a thread that counts must not stand still for that time."""
+    optim = _optim()
+    a = torch.randn(8192, 8192, device='cuda', dtype=torch.bfloat16) * 0.01
+    b = torch.empty_like(a)
+    g = torch.randn(1000, device='cuda')
+    optim.clip_grads_([g], 1e9, error_if_nonfinite=True)
+    torch.mm(a, a, out=b)
+    torch.cuda.synchronize()
+    ticks, stop = [], threading.Event()
+
+    def count():
+        while not stop.is_set():
+            ticks.append(time.perf_counter())
+            time.sleep(0.001)
+
+    t = threading.Thread(target=count)
+    t.start()
+    try:
+        for _ in range(400):                              # a queue of some hundred milliseconds
+            torch.mm(a, a, out=b)
+        start = time.perf_counter()
+        optim.clip_grads_([g], 1e9, error_if_nonfinite=True)
+        end = time.perf_counter()
+    finally:
+        stop.set()
+        t.join()
+    assert end - start > 0.05, end - start                # there was something to wait for
+    inside = [x for x in ticks if start < x < end]
+    gaps = [q - p for p, q in zip([start] + inside, inside + [end])]
+    assert max(gaps) < 0.5 * (end - start), (max(gaps), end - start)

@@ -235,10 +235,38 @@ __global__ __launch_bounds__(256) void adam_clipped_kernel(const AdamArgs d, con
 
 int blocks_for(int64_t chunks) { return (int)(chunks < MAX_BLOCKS ? chunks : MAX_BLOCKS); }
 
+// Order in which the ranges are walked: as given while all of them are within reach of each other (32 bits of distance in elements of 2
+// bytes), else by address, so that a launch ends where the next 4 GiB begin and not wherever the list jumps there and back.
+struct Order {
+    std::vector<int32_t> by_address;      // empty: as given
+    int operator[](int i) const { return by_address.empty() ? i : by_address[i]; }
+    int make(const dsaspp_clip_desc& d, const char* who) {
+        auto at = [&](int i) { return (uintptr_t)d.ranges[i].p; };
+        if (d.n_ranges == 0) return 0;
+        uintptr_t lo = at(0), hi = lo;
+        bool sorted = true;
+        for (int i = 1; i < d.n_ranges; ++i) {
+            sorted = sorted && at(i) >= at(i - 1);
+            lo = std::min(lo, at(i));
+            hi = std::max(hi, at(i));
+        }
+        if (sorted || hi - lo < (1ull << 32)) return 0;
+        try {
+            by_address.resize(d.n_ranges);
+        } catch (const std::bad_alloc&) {
+            dsaspp_set_error("%s: out of host memory", who);
+            return 1;
+        }
+        for (int i = 0; i < d.n_ranges; ++i) by_address[i] = i;
+        std::sort(by_address.begin(), by_address.end(), [&](int a, int b) { return at(a) < at(b) || (at(a) == at(b) && a < b); });
+        return 0;
+    }
+};
+
 // Calls fn(dtype, group) for every launch the ranges need: up to MAX_RANGES ranges of one type each.  A range that begins where
 // the one before it ends goes on with it: gradients that are views of one arena.
 template <typename F>
-void for_each_group(const dsaspp_clip_desc& d, F fn) {
+void for_each_group(const dsaspp_clip_desc& d, const Order& order, F fn) {
     for (int dt = 0; dt < 3; ++dt) {
         const int64_t size = dt == 1 ? 4 : 2;
         Group g;
@@ -253,9 +281,10 @@ void for_each_group(const dsaspp_clip_desc& d, F fn) {
             end = nullptr;
         };
         for (int i = 0; i < d.n_ranges; ++i) {
-            if (d.ranges[i].dtype != dt) continue;
-            char* p = (char*)d.ranges[i].p;
-            for (int64_t left = d.ranges[i].n; left > 0;) {
+            const dsaspp_grad_range& range = d.ranges[order[i]];
+            if (range.dtype != dt) continue;
+            char* p = (char*)range.p;
+            for (int64_t left = range.n; left > 0;) {
                 const int64_t n = left < MAX_LENGTH ? left : MAX_LENGTH, more = (n + CHUNK - 1) / CHUNK;
                 const int k = g.n_ranges - 1;
                 if (k >= 0 && end == p && g.n[k] + n <= MAX_LENGTH && chunks + more <= MAX_CHUNKS) {
@@ -295,9 +324,9 @@ int check(const dsaspp_clip_desc* d, const char* who) {
     return 0;
 }
 
-int64_t n_partials(const dsaspp_clip_desc& d) {
+int64_t n_partials(const dsaspp_clip_desc& d, const Order& order) {
     int64_t n = 0;
-    for_each_group(d, [&](int, const Group& g) { n += blocks_for(g.first[g.n_ranges]); });
+    for_each_group(d, order, [&](int, const Group& g) { n += blocks_for(g.first[g.n_ranges]); });
     return n;
 }
 
@@ -307,15 +336,16 @@ int check_used(const dsaspp_clip_desc* d, const char* who, int64_t used) {
     return 0;
 }
 
-int check_ws(const dsaspp_clip_desc* d, const char* who, int64_t* used) {
+int check_ws(const dsaspp_clip_desc* d, const char* who, Order* order, int64_t* used) {
     if (int rc = check(d, who)) return rc;
-    *used = n_partials(*d);
+    if (int rc = order->make(*d, who)) return rc;
+    *used = n_partials(*d, *order);
     return check_used(d, who, *used);
 }
 
-void launch_partials(const dsaspp_clip_desc& d, hipStream_t s) {
+void launch_partials(const dsaspp_clip_desc& d, const Order& order, hipStream_t s) {
     double* ws = d.ws;
-    for_each_group(d, [&](int dt, const Group& g) {
+    for_each_group(d, order, [&](int dt, const Group& g) {
         const int nb = blocks_for(g.first[g.n_ranges]);
 #define PARTIALS(DT)                                                                                                       \
         if (d.norm_type == 2) hipLaunchKernelGGL((partials_kernel<DT, false>), dim3(nb), dim3(256), 0, s, g, ws);          \
@@ -326,8 +356,8 @@ void launch_partials(const dsaspp_clip_desc& d, hipStream_t s) {
     });
 }
 
-void launch_scale(const dsaspp_clip_desc& d, int used, hipStream_t s) {
-    for_each_group(d, [&](int dt, const Group& g) {
+void launch_scale(const dsaspp_clip_desc& d, const Order& order, int used, hipStream_t s) {
+    for_each_group(d, order, [&](int dt, const Group& g) {
         const int nb = blocks_for(g.first[g.n_ranges]);
         if (dt == 0) hipLaunchKernelGGL(scale_kernel<0>, dim3(nb), dim3(256), 0, s, g, d.ws, used, d.norm_type, d.max_norm, d.norm);
         else if (dt == 1) hipLaunchKernelGGL(scale_kernel<1>, dim3(nb), dim3(256), 0, s, g, d.ws, used, d.norm_type, d.max_norm, d.norm);
@@ -397,21 +427,24 @@ extern "C" int dsaspp_grad_ranges_overlap(const dsaspp_clip_desc* d) {
 }
 
 extern "C" int64_t dsaspp_grad_norm_workspace(const dsaspp_clip_desc* d) {
-    if (check(d, "grad_norm_workspace")) return -1;
-    return n_partials(*d);
+    Order order;
+    if (check(d, "grad_norm_workspace") || order.make(*d, "grad_norm_workspace")) return -1;
+    return n_partials(*d, order);
 }
 
 extern "C" int dsaspp_grad_norm_partials(const dsaspp_clip_desc* d, dsaspp_stream_t stream) {
     int64_t used = 0;
-    if (int rc = check_ws(d, "grad_norm_partials", &used)) return rc;
-    launch_partials(*d, (hipStream_t)stream);
+    Order order;
+    if (int rc = check_ws(d, "grad_norm_partials", &order, &used)) return rc;
+    launch_partials(*d, order, (hipStream_t)stream);
     DS_LAUNCH_CHECK("grad_norm_partials");
     return 0;
 }
 
 extern "C" int dsaspp_grad_norm_finish(const dsaspp_clip_desc* d, dsaspp_stream_t stream) {
     int64_t used = 0;
-    if (int rc = check_ws(d, "grad_norm_finish", &used)) return rc;
+    Order order;
+    if (int rc = check_ws(d, "grad_norm_finish", &order, &used)) return rc;
     DS_REQUIRE(d->norm, "grad_norm_finish: null output");
     hipLaunchKernelGGL(finish_kernel, dim3(1), dim3(256), 0, (hipStream_t)stream, d->ws, (int)used, d->norm_type, d->scale, d->norm);
     DS_LAUNCH_CHECK("grad_norm_finish");
@@ -420,22 +453,25 @@ extern "C" int dsaspp_grad_norm_finish(const dsaspp_clip_desc* d, dsaspp_stream_
 
 extern "C" int dsaspp_clip_scale(const dsaspp_clip_desc* d, dsaspp_stream_t stream) {
     int64_t used = 0;
-    if (int rc = check_ws(d, "clip_scale", &used)) return rc;
+    Order order;
+    if (int rc = check_ws(d, "clip_scale", &order, &used)) return rc;
     DS_REQUIRE(d->norm, "clip_scale: null output");
     DS_REQUIRE(d->scale == 1.f, "clip_scale: scale must be 1");
     DS_REQUIRE(d->max_norm >= 0.f, "clip_scale: max_norm must be >= 0");
     if (d->n_ranges == 0) return dsaspp_grad_norm_finish(d, stream);
-    launch_scale(*d, (int)used, (hipStream_t)stream);
+    launch_scale(*d, order, (int)used, (hipStream_t)stream);
     DS_LAUNCH_CHECK("clip_scale");
     return 0;
 }
 
 extern "C" int dsaspp_clip_grads(const dsaspp_clip_desc* d, dsaspp_stream_t stream) {
+    Order order;
     if (int rc = check(d, "clip_grads")) return rc;
+    if (int rc = order.make(*d, "clip_grads")) return rc;
     DS_REQUIRE(d->norm && d->scale == 1.f && d->max_norm >= 0.f, "clip_grads: null output, scale other than 1 or negative max_norm");
     int64_t total = 0, used = 0;
     int groups = 0, ranges = 0;
-    for_each_group(*d, [&](int, const Group& g) {
+    for_each_group(*d, order, [&](int, const Group& g) {
         ++groups;
         ranges += g.n_ranges;
         used += blocks_for(g.first[g.n_ranges]);
@@ -445,14 +481,14 @@ extern "C" int dsaspp_clip_grads(const dsaspp_clip_desc* d, dsaspp_stream_t stre
     hipStream_t s = (hipStream_t)stream;
     if (groups == 0) return dsaspp_grad_norm_finish(d, stream);
     if (groups == 1 && ranges <= ONE_BLOCK_RANGES && total <= ONE_BLOCK) {
-        for_each_group(*d, [&](int dt, const Group& g) {
+        for_each_group(*d, order, [&](int dt, const Group& g) {
             if (dt == 0) hipLaunchKernelGGL(clip_one_kernel<0>, dim3(1), dim3(1024), 0, s, g, d->norm_type, d->max_norm, d->norm);
             else if (dt == 1) hipLaunchKernelGGL(clip_one_kernel<1>, dim3(1), dim3(1024), 0, s, g, d->norm_type, d->max_norm, d->norm);
             else hipLaunchKernelGGL(clip_one_kernel<2>, dim3(1), dim3(1024), 0, s, g, d->norm_type, d->max_norm, d->norm);
         });
     } else {
-        launch_partials(*d, s);
-        launch_scale(*d, (int)used, s);
+        launch_partials(*d, order, s);
+        launch_scale(*d, order, (int)used, s);
     }
     DS_LAUNCH_CHECK("clip_grads");
     return 0;
@@ -460,11 +496,12 @@ extern "C" int dsaspp_clip_grads(const dsaspp_clip_desc* d, dsaspp_stream_t stre
 
 extern "C" int dsaspp_adam_step_clipped(const dsaspp_adam_clip_desc* a, const dsaspp_clip_desc* c, dsaspp_stream_t stream) {
     int64_t used = 0;
+    Order order;
     DS_REQUIRE(a && a->n > 0 && a->n <= MAX_ELEMS, "adam_step_clipped: n must be positive");
     DS_REQUIRE(a->p && a->g && a->m && a->v && a->step >= 1, "adam_step_clipped: bad descriptor");
     DS_REQUIRE((((uintptr_t)a->p | (uintptr_t)a->g | (uintptr_t)a->m | (uintptr_t)a->v) & 3) == 0 && ((uintptr_t)a->w16 & 1) == 0,
                "adam_step_clipped: buffers must be aligned to their element type");
-    if (int rc = check_ws(c, "adam_step_clipped", &used)) return rc;
+    if (int rc = check_ws(c, "adam_step_clipped", &order, &used)) return rc;
     DS_REQUIRE(c->norm && c->max_norm >= 0.f, "adam_step_clipped: null output or negative max_norm");
     const AdamArgs d = {a->n, a->p, a->g, a->m, a->v, reinterpret_cast<u16*>(a->w16),
                         (float)(a->lr / (1.0 - pow(a->beta1, (double)a->step))), (float)a->beta1, (float)(1.0 - a->beta1), (float)a->beta2,

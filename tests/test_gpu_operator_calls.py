@@ -1,13 +1,16 @@
 """-m gpu: calls of the class-score and gradient-norm operators beside the usual ones."""
+import math
 import threading
 import time
 
 import pytest
 import torch
 
+import scores_ref as R
 from test_gpu_scores import _tiny
 
 pytestmark = pytest.mark.gpu
+U = R.U
 
 
 def _optim():
@@ -64,3 +67,21 @@ def test_other_threads_run_while_a_call_waits_for_the_norm():
     inside = [x for x in ticks if start < x < end]
     gaps = [q - p for p, q in zip([start] + inside, inside + [end])]
     assert max(gaps) < 0.5 * (end - start), (max(gaps), end - start)
+
+
+def test_gradients_in_far_apart_allocations():
+    """16-bit gradients on either side of 4 GB, given in turn: the norm and the scaled values are those of the list."""
+    optim = _optim()
+    arena = torch.empty(3 * 2 ** 30, dtype=torch.bfloat16, device='cuda')
+    g = torch.Generator().manual_seed(3)
+    z = [torch.randn(1003, generator=g).to(torch.bfloat16) for _ in range(8)]
+    at = [(2 ** 31 + 2 ** 29) * (i % 2) + 5000 * i + 1 for i in range(8)]
+    ts = [arena[a:a + 1003] for a in at]
+    for t, s in zip(ts, z):
+        t.copy_(s)
+    want = math.sqrt(sum(float(s.double().square().sum()) for s in z))
+    assert abs(float(optim.grad_norm(ts)) - want) <= 1.01 * U * want
+    optim.clip_grads_(ts, 1.0)
+    for t, s in zip(ts, z):
+        b = s.double() / (want + 1e-6)
+        R.agree(t, b, 3 * U * b.abs(), 'clipped', torch.bfloat16)

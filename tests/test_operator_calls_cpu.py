@@ -1,4 +1,6 @@
 """Calls around the class-score and gradient-norm operators whose outcome shows without a GPU."""
+import ctypes
+
 import pytest
 import torch
 import torch.autograd.forward_ad as fwad
@@ -6,7 +8,7 @@ import torch.autograd.forward_ad as fwad
 import denseASPP  # noqa: F401
 import kernel_model
 from e2e_common import TINY_CFG, make_batch, make_pair
-from semantic_segmentation_amd import label_scores, optim
+from semantic_segmentation_amd import _lib, label_scores, optim
 
 
 @pytest.fixture
@@ -68,3 +70,23 @@ def test_tracing_is_refused(fp32_model):
                   (lambda a: optim.adam_update_(a, a, a, a, 1), z), (lambda a: mod.score(a).entropy, torch.randn(1, 3, 64, 64))):
         with pytest.raises(RuntimeError, match='traced'):
             torch.jit.trace(fn, (x,))
+
+
+def _workspace(addresses, n):
+    arr = (_lib.grad_range * len(addresses))()
+    for r, p in zip(arr, addresses):
+        r.p, r.n, r.dtype = p, n, 0
+    d = _lib.clip_desc()
+    d.ranges, d.n_ranges, d.norm_type, d.scale = ctypes.cast(arr, ctypes.c_void_p), len(addresses), 2, 1.0
+    return _lib.load().dsaspp_grad_norm_workspace(ctypes.byref(d))
+
+
+def test_launches_do_not_depend_on_the_order_of_the_list():
+    """A launch of large ranges has as many partials as blocks, 2048; ranges 8 GB apart cannot share one.  Given in turn they make as many
+    launches as given one side after the other."""
+    n = 10_000_000
+    near = [(1 << 40) + i * (1 << 25) for i in range(5)]
+    far = [a + (1 << 33) for a in near]
+    turn = [a for pair in zip(near, far) for a in pair]
+    assert _workspace(near, n) == 2048
+    assert _workspace(turn, n) == _workspace(near + far, n) == _workspace(far[::-1] + near, n) == 2 * 2048

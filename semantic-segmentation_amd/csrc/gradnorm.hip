@@ -240,24 +240,16 @@ int blocks_for(int64_t chunks) { return (int)(chunks < MAX_BLOCKS ? chunks : MAX
 struct Order {
     std::vector<int32_t> by_address;      // empty: as given
     int operator[](int i) const { return by_address.empty() ? i : by_address[i]; }
-    int make(const dsaspp_clip_desc& d, const char* who) {
-        auto at = [&](int i) { return (uintptr_t)d.ranges[i].p; };
-        if (d.n_ranges == 0) return 0;
-        uintptr_t lo = at(0), hi = lo;
-        bool sorted = true;
-        for (int i = 1; i < d.n_ranges; ++i) {
-            sorted = sorted && at(i) >= at(i - 1);
-            lo = std::min(lo, at(i));
-            hi = std::max(hi, at(i));
-        }
+    // lo, hi: of the ranges' addresses; sorted: they ascend
+    int make(const dsaspp_clip_desc& d, const char* who, uintptr_t lo, uintptr_t hi, bool sorted) {
         if (sorted || hi - lo < (1ull << 32)) return 0;
         try {
             by_address.resize(d.n_ranges);
         } catch (const std::bad_alloc&) {
-            dsaspp_set_error("%s: out of host memory", who);
-            return 1;
+            return dsaspp_set_error("%s: out of host memory", who);
         }
         for (int i = 0; i < d.n_ranges; ++i) by_address[i] = i;
+        auto at = [&](int i) { return (uintptr_t)d.ranges[i].p; };
         std::sort(by_address.begin(), by_address.end(), [&](int a, int b) { return at(a) < at(b) || (at(a) == at(b) && a < b); });
         return 0;
     }
@@ -310,18 +302,25 @@ void for_each_group(const dsaspp_clip_desc& d, const Order& order, F fn) {
     }
 }
 
-int check(const dsaspp_clip_desc* d, const char* who) {
+int check(const dsaspp_clip_desc* d, const char* who, Order* order = nullptr) {
     DS_REQUIRE(d, "%s: null descriptor", who);
     DS_REQUIRE(d->n_ranges >= 0 && (d->n_ranges == 0 || d->ranges), "%s: bad list of ranges", who);
     DS_REQUIRE(d->norm_type == 2 || d->norm_type == 0, "%s: norm_type must be 2 (Euclidean) or 0 (largest magnitude), got %d", who, d->norm_type);
     DS_REQUIRE(d->scale > 0.f && d->scale < INFINITY, "%s: scale must be positive and finite", who);
+    uintptr_t lo = UINTPTR_MAX, hi = 0, last = 0;
+    bool sorted = true;
     for (int i = 0; i < d->n_ranges; ++i) {
         const dsaspp_grad_range& r = d->ranges[i];
+        const uintptr_t p = (uintptr_t)r.p;
+        lo = std::min(lo, p);
+        hi = std::max(hi, p);
+        sorted = sorted && p >= last;
+        last = p;
         DS_REQUIRE(r.dtype >= 0 && r.dtype <= 2, "%s: range %d has dtype %d (0 = bf16, 1 = fp32, 2 = fp16)", who, i, r.dtype);
         DS_REQUIRE(r.p && r.n > 0 && r.n <= MAX_ELEMS, "%s: range %d is empty, too long or null", who, i);
         DS_REQUIRE(((uintptr_t)r.p & (r.dtype == 1 ? 3 : 1)) == 0, "%s: range %d is not aligned to its element type", who, i);
     }
-    return 0;
+    return order ? order->make(*d, who, lo, hi, sorted) : 0;
 }
 
 int64_t n_partials(const dsaspp_clip_desc& d, const Order& order) {
@@ -337,8 +336,7 @@ int check_used(const dsaspp_clip_desc* d, const char* who, int64_t used) {
 }
 
 int check_ws(const dsaspp_clip_desc* d, const char* who, Order* order, int64_t* used) {
-    if (int rc = check(d, who)) return rc;
-    if (int rc = order->make(*d, who)) return rc;
+    if (int rc = check(d, who, order)) return rc;
     *used = n_partials(*d, *order);
     return check_used(d, who, *used);
 }
@@ -428,7 +426,7 @@ extern "C" int dsaspp_grad_ranges_overlap(const dsaspp_clip_desc* d) {
 
 extern "C" int64_t dsaspp_grad_norm_workspace(const dsaspp_clip_desc* d) {
     Order order;
-    if (check(d, "grad_norm_workspace") || order.make(*d, "grad_norm_workspace")) return -1;
+    if (check(d, "grad_norm_workspace", &order)) return -1;
     return n_partials(*d, order);
 }
 
@@ -466,8 +464,7 @@ extern "C" int dsaspp_clip_scale(const dsaspp_clip_desc* d, dsaspp_stream_t stre
 
 extern "C" int dsaspp_clip_grads(const dsaspp_clip_desc* d, dsaspp_stream_t stream) {
     Order order;
-    if (int rc = check(d, "clip_grads")) return rc;
-    if (int rc = order.make(*d, "clip_grads")) return rc;
+    if (int rc = check(d, "clip_grads", &order)) return rc;
     DS_REQUIRE(d->norm && d->scale == 1.f && d->max_norm >= 0.f, "clip_grads: null output, scale other than 1 or negative max_norm");
     int64_t total = 0, used = 0;
     int groups = 0, ranges = 0;

@@ -641,7 +641,9 @@ int dsaspp_adam_step(const dsaspp_adam_desc* d, dsaspp_stream_t stream);
  *   coef = min(1, max_norm / (norm + 1e-6))           a NaN norm gives a NaN coefficient
  * The gradients are a HOST array of dense device ranges; it is read during the call only and may be freed after it.  A range
  * needs no more alignment than its element type.  Sums are fp64 (the square of an fp32 value is exact there and cannot overflow) and
- * taken in an order that depends on the list of sizes alone, so equal lists give equal bits.
+ * taken in an order that depends on the list alone -- sizes, types, addresses (ranges that follow one another in memory are one) and their
+ * order: the same list gives the same bits each time.  Equal values elsewhere in memory may be added up in another order: their norm may be
+ * another last bit away.
  *   1. dsaspp_grad_norm_partials: one fp64 partial per block into ws (dsaspp_grad_norm_workspace doubles, contents need not be
  *      initialised).  n_ranges == 0 is allowed: the norm is 0.
  *   2. dsaspp_grad_norm_finish: norm[0] from the partials; or

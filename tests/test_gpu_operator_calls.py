@@ -85,3 +85,21 @@ def test_gradients_in_far_apart_allocations():
     for t, s in zip(ts, z):
         b = s.double() / (want + 1e-6)
         R.agree(t, b, 3 * U * b.abs(), 'clipped', torch.bfloat16)
+
+
+def test_equal_values_laid_out_otherwise():
+    """Adjacent, apart and in one piece: the sums are taken in other orders, each in fp64, and every norm is within its own rounding of the
+    same value; the same list gives the same bits."""
+    optim = _optim()
+    g = torch.Generator().manual_seed(8)
+    z = [torch.randn(n, generator=g) for n in (5000, 3, 4097, 20000, 8192)]
+    want = math.sqrt(sum(float(s.double().square().sum()) for s in z))
+    flat = torch.cat(z).cuda()
+    views, at = [], 0
+    for s in z:
+        views.append(flat[at:at + s.numel()])
+        at += s.numel()
+    for ts in (views, [flat], [s.cuda() for s in z], [torch.cat((s, s[:1])).cuda()[:-1] for s in z]):
+        first = optim.grad_norm(ts)
+        assert abs(float(first) - want) <= 1.01 * U * want
+        assert all(torch.equal(optim.grad_norm(ts), first) for _ in range(3))

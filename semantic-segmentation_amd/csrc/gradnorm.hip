@@ -125,12 +125,25 @@ __device__ __forceinline__ double total_norm(const double* ws, int n, float scal
     return (double)scale * (MAXNORM ? v : sqrt(v));
 }
 
-__device__ __forceinline__ float clip_coef(double norm, float max_norm) {
+__device__ __forceinline__ double clip_coef(double norm, float max_norm) {
     // an infinite threshold never clips (inf / inf would be NaN); a NaN norm stays NaN
-    if (norm == norm && max_norm == INFINITY) return 1.f;
+    if (norm == norm && max_norm == INFINITY) return 1.0;
     const double c = (double)max_norm / (norm + 1e-6);
-    return c > 1.0 ? 1.f : (float)c;
+    return c > 1.0 ? 1.0 : c;
 }
+
+// A factor for fp32 values, rounded once to 24 bits: below 2^-100 in two, as one it would lose its last bits as a denormal (a norm of 1e39
+// clipped to 1) while the values it multiplies are large.
+struct Factor {
+    float a, b;
+    __device__ __forceinline__ explicit Factor(double c) {
+        const bool small = c < 0x1p-100;                  // false for NaN
+        a = (float)(small ? c * 0x1p100 : c);
+        b = small ? 0x1p-100f : 1.f;
+    }
+    __device__ __forceinline__ float times(float x) const { return x * a * b; }
+    __device__ __forceinline__ bool one() const { return a == 1.f && b == 1.f; }
+};
 
 __device__ __forceinline__ double any_norm(const double* ws, int n, int norm_type, float scale, double* lds) {
     return norm_type == 2 ? total_norm<false>(ws, n, scale, lds) : total_norm<true>(ws, n, scale, lds);
@@ -148,8 +161,8 @@ __global__ __launch_bounds__(256) void scale_kernel(const Group g, const double*
     __shared__ double lds[4];
     const double total = any_norm(ws, n_ws, norm_type, 1.f, lds);
     if (blockIdx.x == 0 && threadIdx.x == 0) norm[0] = (float)total;
-    const float coef = clip_coef(total, max_norm);
-    if (coef == 1.f) return;              // x * 1 is x
+    const Factor coef(clip_coef(total, max_norm));
+    if (coef.one()) return;               // x * 1 is x
     const int n_chunks = g.first[g.n_ranges];
     const Share sh = share_of(n_chunks);
     int r = find_range(g, sh.last - 1);
@@ -167,7 +180,7 @@ __global__ __launch_bounds__(256) void scale_kernel(const Group g, const double*
 #pragma unroll
             for (int it = 0; it < IT; ++it) {
 #pragma unroll
-                for (int k = 0; k < E::N; ++k) v[it][k] = E::down(E::up(v[it][k]) * coef);
+                for (int k = 0; k < E::N; ++k) v[it][k] = E::down(coef.times(E::up(v[it][k])));
                 *reinterpret_cast<typename E::V*>(p + i + it * 256 * E::N) = v[it];
             }
         }
@@ -175,11 +188,11 @@ __global__ __launch_bounds__(256) void scale_kernel(const Group g, const double*
             typename E::V* q = reinterpret_cast<typename E::V*>(p + i);
             typename E::V v = *q;
 #pragma unroll
-            for (int k = 0; k < E::N; ++k) v[k] = E::down(E::up(v[k]) * coef);
+            for (int k = 0; k < E::N; ++k) v[k] = E::down(coef.times(E::up(v[k])));
             *q = v;
         }
         const int t = n / E::N * E::N + (int)threadIdx.x;
-        if (t < n) p[t] = E::down(E::up(p[t]) * coef);
+        if (t < n) p[t] = E::down(coef.times(E::up(p[t])));
     }
 }
 
@@ -196,9 +209,9 @@ __global__ __launch_bounds__(256) void adam_clipped_kernel(const AdamArgs d, con
     __shared__ double lds[4];
     const double total = any_norm(ws, n_ws, norm_type, scale, lds);
     if (blockIdx.x == 0 && threadIdx.x == 0) norm[0] = (float)total;
-    const float gs = scale * clip_coef(total, max_norm);
+    const Factor gs((double)scale * clip_coef(total, max_norm));
     auto update = [&](float& p, const float gr, float& m, float& v) {
-        const float g = gr * gs + d.weight_decay * p;
+        const float g = gs.times(gr) + d.weight_decay * p;
         m = d.beta1 * m + d.beta1c * g;
         v = d.beta2 * v + d.beta2c * g * g;
         p -= d.lr1 * (m / (sqrtf(v) / d.bc2s + d.eps));
@@ -394,12 +407,12 @@ __global__ __launch_bounds__(1024) void clip_one_kernel(const Group g, int norm_
     for (int w = 1; w < 16; ++w) acc = norm_type == 2 ? acc + lds[w] : join<true>(acc, lds[w]);
     const double total = norm_type == 2 ? sqrt(acc) : acc;
     if (threadIdx.x == 0) norm[0] = (float)total;
-    const float coef = clip_coef(total, max_norm);
-    if (coef == 1.f) return;
+    const Factor coef(clip_coef(total, max_norm));
+    if (coef.one()) return;
     for (int r = 0; r < g.n_ranges; ++r) {
         typename E::T* p = reinterpret_cast<typename E::T*>(g.base) + g.at[r];
         const int n = (int)g.n[r];
-        for (int i = threadIdx.x; i < n; i += 1024) p[i] = E::down(E::up(p[i]) * coef);
+        for (int i = threadIdx.x; i < n; i += 1024) p[i] = E::down(coef.times(E::up(p[i])));
     }
 }
 

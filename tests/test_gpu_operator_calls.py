@@ -103,3 +103,23 @@ def test_equal_values_laid_out_otherwise():
         first = optim.grad_norm(ts)
         assert abs(float(first) - want) <= 1.01 * U * want
         assert all(torch.equal(optim.grad_norm(ts), first) for _ in range(3))
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('n', [1000, 300_001])
+def test_coefficients_below_the_normal_range(n, dtype):
+    """A norm of 3e36 and more clipped to thresholds that make the coefficient itself a denormal or 0 in fp32."""
+    optim = _optim()
+    z = (torch.randn(n, generator=torch.Generator().manual_seed(n)) * 1e35).to(dtype)
+    for max_norm in (1.0, 1e-3, 1e-6):
+        t = z.cuda()
+        want = float(z.double().norm())
+        coef = max_norm / (want + 1e-6)
+        assert abs(float(optim.clip_grads_([t], max_norm)) - want) <= 1.01 * U * want
+        b = z.double() * coef
+        R.agree(t, b, 3 * U * b.abs(), 'clipped', dtype)
+    if dtype == torch.float32:                            # the same coefficient inside the Adam update
+        p, m, v = (torch.zeros(n, device='cuda') for _ in range(3))
+        optim.adam_update_(p, z.cuda(), m, v, 1, lr=1.0, betas=(0.5, 0.5), eps=1.0, max_grad_norm=1e-3)
+        b = z.double() * (1e-3 / (want + 1e-6))
+        R.agree(m, 0.5 * b, 6 * U * (0.5 * b).abs(), 'first moment')

@@ -121,13 +121,10 @@ class FusedAdam:
         self._moments()
         if grad_scale is None:
             grad_scale = getattr(mod, '_grad_scale', 1.0)
-        # the scale a GradReducer left belongs to the gradients of THAT backward pass: used once, then back to 1, so
-        # that a later step on locally computed gradients (train_step without a reducer, loss.backward()) is not scaled
-        mod._grad_scale = 1.0
         g0 = mod._first_param.grad
         if g0 is None or g0.data_ptr() != mod._gflat.data_ptr() + 4 * mod.arena.by_name[mod._param_names[0]].off:
             mod.sync_grads_to_arena()         # gradients came from loss.backward() through model(x), not from train_step
-        self.step_count += 1
+        step = self.step_count + 1            # counted once the update has been launched: a refused one changes nothing
         lib = _lib.load()
         g = self.param_groups[0]
         # fp32 compute mode: the "shadow" IS the master arena (the fp32 kernels read it directly); writing packed bf16
@@ -135,10 +132,11 @@ class FusedAdam:
         shadow_is_master = mod._w16 is None or mod._w16.data_ptr() == flat.data_ptr() or mod._w16.dtype != torch.bfloat16
         if max_grad_norm is not None:
             with torch.cuda.device(flat.device):
-                norm = adam_update_(flat, mod._gflat, self.m, self.v, self.step_count, lr=float(g['lr']), betas=g.get('betas', self.betas),
+                norm = adam_update_(flat, mod._gflat, self.m, self.v, step, lr=float(g['lr']), betas=g.get('betas', self.betas),
                                     eps=float(g.get('eps', self.eps)), weight_decay=float(g.get('weight_decay', self.weight_decay)),
                                     grad_scale=float(grad_scale), max_grad_norm=float(max_grad_norm),
                                     shadow=None if shadow_is_master else mod._w16)
+                self._counted(step)
                 mod._get_backend().refresh_weights(mod, cast=shadow_is_master)
             mod._weights_fresh = True
             return norm
@@ -149,12 +147,19 @@ class FusedAdam:
         d.lr = float(g['lr'])
         d.beta1, d.beta2 = g.get('betas', self.betas)
         d.eps, d.weight_decay = float(g.get('eps', self.eps)), float(g.get('weight_decay', self.weight_decay))
-        d.step = self.step_count
+        d.step = step
         d.grad_scale = float(grad_scale)
         stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
         _lib.check(lib.dsaspp_adam_step(ctypes.byref(d), stream))
+        self._counted(step)
         mod._get_backend().refresh_weights(mod, cast=shadow_is_master)
         mod._weights_fresh = True
+
+    def _counted(self, step):
+        self.step_count = step
+        # the scale a GradReducer left belongs to the gradients of THAT backward pass: used once, then back to 1, so
+        # that a later step on locally computed gradients (train_step without a reducer, loss.backward()) is not scaled
+        self.model._grad_scale = 1.0
 
     # ------------------------------------------------------------------ checkpoint format of torch.optim.Adam
     def state_dict(self):

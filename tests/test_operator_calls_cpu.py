@@ -90,3 +90,21 @@ def test_launches_do_not_depend_on_the_order_of_the_list():
     turn = [a for pair in zip(near, far) for a in pair]
     assert _workspace(near, n) == 2048
     assert _workspace(turn, n) == _workspace(near + far, n) == _workspace(far[::-1] + near, n) == 2 * 2048
+
+
+def test_a_refused_update_leaves_the_optimizer_as_it_was(monkeypatch):
+    _, mod = _pair()
+    opt = optim.FusedAdam(mod)
+    mod._grad_scale = 0.25                                 # as a reducer leaves it
+
+    def refuse(*a, **k):
+        raise ValueError('refused')
+
+    monkeypatch.setattr(torch.cuda, 'device', lambda d: torch.enable_grad())
+    monkeypatch.setattr(optim, 'adam_update_', refuse)
+    with pytest.raises(ValueError, match='refused'):
+        opt.step(max_grad_norm=1.0)
+    assert opt.step_count == 0 and mod._grad_scale == 0.25
+    monkeypatch.setattr(optim, 'adam_update_', lambda p, g, m, v, step, **k: torch.tensor(float(step) * k['grad_scale']))
+    assert float(opt.step(max_grad_norm=1.0)) == 0.25
+    assert opt.step_count == 1 and mod._grad_scale == 1.0

@@ -546,7 +546,8 @@ Tensor adam_update(const Tensor& p, const Tensor& grad, const Tensor& m, const T
         VALUE_CHECK(t->is_cuda() && t->scalar_type() == at::kFloat && t->numel() == p.numel() && t->device() == p.device() && t->is_contiguous() && !t->is_neg(),
                     "adam_update_ needs contiguous float32 tensors of one size on one GPU");
     if (shadow.has_value())
-        VALUE_CHECK(shadow->scalar_type() == at::kBFloat16 && shadow->numel() == p.numel() && shadow->device() == p.device() && shadow->is_contiguous(),
+        VALUE_CHECK(shadow->scalar_type() == at::kBFloat16 && shadow->numel() == p.numel() && shadow->device() == p.device() && shadow->is_contiguous() &&
+                        !shadow->is_neg(),
                     "adam_update_: shadow must be a contiguous bfloat16 tensor of the size of param");
     VALUE_CHECK(p.numel() > 0, "adam_update_ needs at least one element");
     std::vector<std::pair<char*, char*>> spans;

@@ -123,3 +123,11 @@ def test_coefficients_below_the_normal_range(n, dtype):
         optim.adam_update_(p, z.cuda(), m, v, 1, lr=1.0, betas=(0.5, 0.5), eps=1.0, max_grad_norm=1e-3)
         b = z.double() * (1e-3 / (want + 1e-6))
         R.agree(m, 0.5 * b, 6 * U * (0.5 * b).abs(), 'first moment')
+
+
+def test_negated_shadow_is_refused():
+    optim = _optim()
+    p, g, m, v = (torch.zeros(8, device='cuda') for _ in range(4))
+    shadow = torch._neg_view(torch.zeros(8, device='cuda', dtype=torch.bfloat16))
+    with pytest.raises(ValueError, match='shadow'):
+        optim.adam_update_(p, g, m, v, 1, shadow=shadow)

@@ -498,12 +498,15 @@ class DenseASPP(nn.Module):
         scores.label_scores gives them -- log probability of `labels` (int64, N x H x W; 0 at ignore_index), entropy, and the top_k
         classes with their log probabilities -- computed from the low-resolution logits without the upsampled ones.
         In train() mode with gradients enabled the result is differentiable with respect to the parameters (and to x), so a
-        loss of one's own trains the network: loss.backward(), then any optimizer."""
+        loss of one's own trains the network: loss.backward(), then any optimizer.  Not for capture into a graph."""
         if x.dim() != 4 or x.shape[1] != 3:
             raise ValueError('DenseASPP expects an N x 3 x H x W image batch, got %s' % (tuple(x.shape),))
         if x.shape[2] % 8 or x.shape[3] % 8:
             raise ValueError('DenseASPP.score: H and W must be multiples of 8, got %d x %d' % tuple(x.shape[2:]))
         _lib.binding().check_image(x)
+        if x.is_cuda and torch.cuda.is_current_stream_capturing():
+            # the network's programs hold memset nodes and a side stream; a replay of the former does not reliably clear
+            raise RuntimeError('DenseASPP.score: a pass of the network cannot be captured into a graph')
         args = (labels, int(top_k), int(ignore_index), bool(entropy))
         # before the pass, which updates running statistics in train() mode
         _lib.binding().check_scores([x.shape[0], self.spec.n_class, x.shape[2] // 8, x.shape[3] // 8], str(x.device), labels, args[1], args[3], 8)

@@ -131,3 +131,14 @@ def test_negated_shadow_is_refused():
     shadow = torch._neg_view(torch.zeros(8, device='cuda', dtype=torch.bfloat16))
     with pytest.raises(ValueError, match='shadow'):
         optim.adam_update_(p, g, m, v, 1, shadow=shadow)
+
+
+def test_capture_of_a_network_pass_is_refused(monkeypatch):
+    """Its programs clear memory in ways that a graph does not replay: asked whether that is seen, without a real capture."""
+    _, mod = _tiny(False)
+    x = torch.randn(1, 3, 64, 64, device='cuda')
+    with monkeypatch.context() as m:
+        m.setattr(torch.cuda, 'is_current_stream_capturing', lambda: True)
+        with pytest.raises(RuntimeError, match='captured'):
+            mod.score(x)
+    assert bool(torch.isfinite(mod.score(x).entropy).all())

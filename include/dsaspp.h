@@ -58,7 +58,8 @@ const char* dsaspp_last_error(void);
  *   else         { y[m*ldy+c] = v (bf16, or fp32 when y_f32);
  *                  if (stat_acc) { stat_acc[rep][c] += v_stored; stat_acc[rep][cout+c] += v_stored^2; } }
  * where rep = blockIdx % DSASPP_STAT_REPLICAS and the stat buffers are fp32
- * [DSASPP_STAT_REPLICAS][2*cout].
+ * [DSASPP_STAT_REPLICAS][2*cout]: the sum over all rows counts (the fp32 form adds
+ * 64-bit sums to stat_acc as a value and its rest in two rows).
  */
 typedef struct dsaspp_conv_desc {
     int32_t n_img, H, W;      /* feature-map geometry (input == output) */

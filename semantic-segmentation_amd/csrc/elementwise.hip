@@ -23,7 +23,7 @@ __global__ void bn_finalize_kernel(const dsaspp_bn_desc d) {
     } else {
         const int a = c - d.acc_c0;
         if (d.acc && a >= 0 && a < d.acc_cn) {
-            float s = 0.f, q = 0.f;
+            double s = 0.0, q = 0.0;      // the difference below cancels, and the fp32 form keeps its sums in pairs
             for (int r = 0; r < DS_R; ++r) {
                 float* row = d.acc + (size_t)r * 2 * d.acc_cn;
                 s += row[a];
@@ -31,8 +31,9 @@ __global__ void bn_finalize_kernel(const dsaspp_bn_desc d) {
                 row[a] = 0.f;
                 row[d.acc_cn + a] = 0.f;
             }
-            mean = s / d.count;
-            var = fmaxf(q / d.count - mean * mean, 0.f);
+            const double m = s / d.count;
+            mean = (float)m;
+            var = fmaxf((float)(q / d.count - m * m), 0.f);
             d.mean[c] = mean;
             d.var[c] = var;
             d.rstd[c] = rsqrtf(var + d.eps);

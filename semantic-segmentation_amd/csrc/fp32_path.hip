@@ -161,15 +161,11 @@ __global__ __launch_bounds__(256) void conv_f32_kernel(const dsaspp_conv_desc d,
                 }
             } else {
                 if (ok) *reinterpret_cast<float4*>(yg + pc * d.ldy + qc) = make_float4(v[0], v[1], v[2], v[3]);
-                if (d.stat_acc) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) { s1[e] += v[e]; s2[e] = fmaf(v[e], v[e], s2[e]); }
-                }
             }
         }
         // per-channel sums: over the 16 pixels of the DPP row, then one atomic per channel and row of lanes
-        float* sums = d.s_acc ? d.s_acc : (gg ? nullptr : d.stat_acc);
-        const int half = d.s_acc ? sld : cout;
+        float* sums = d.s_acc;
+        const int half = sld;
         if (sums) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -270,12 +266,41 @@ __global__ __launch_bounds__(256) void wgrad_f32_kernel(const dsaspp_wgrad_desc 
 }
 
 // ---------------------------------------------------------------- row-wise fp32 kernels: a lane owns 4 channels of a pixel
-// statistics of a stored float4 (sum, sum of squares) into replica row `rep` of an accumulator [R][2*C]: one atomic per
-// element -- this path is for checking, not for speed
-__device__ __forceinline__ void stat_add4(float* acc, const int C, const int rep, const int c, const float4 v) {
-    float* a = acc + (size_t)rep * 2 * C + c;
-    atomicAdd(a + 0, v.x); atomicAdd(a + 1, v.y); atomicAdd(a + 2, v.z); atomicAdd(a + 3, v.w);
-    atomicAdd(a + C + 0, v.x * v.x); atomicAdd(a + C + 1, v.y * v.y); atomicAdd(a + C + 2, v.z * v.z); atomicAdd(a + C + 3, v.w * v.w);
+// Statistics (sum, sum of squares) of C channels of M stored pixel rows into an accumulator [R][2*C], in 64 bits and a fixed order: a block has
+// 64 channels of an eighth of the rows, 16 rows at a time, and leaves its sums as fp32 pairs (value, rest) in two replica rows of its own.
+// Sums of fp32 atomics are some 3e-7 off and differ from run to run; that shifts a whole channel, turns the sign of a few pre-activations next to
+// zero, and at random initialisation each of them moves the gradient behind norm5 by some 1e-3 (relative L2).
+constexpr int ST_SPLIT = DS_R / 2, ST_ROWS = 16;
+static_assert(2 * ST_SPLIT == DS_R, "two replica rows per block");
+__global__ __launch_bounds__(64 * ST_ROWS) void stats_f32_kernel(const float* y, const int64_t ld, const int C, const int64_t M, float* acc) {
+    __shared__ double red[2][ST_ROWS][64];
+    const int cl = threadIdx.x & 63, row = threadIdx.x >> 6, c = blockIdx.x * 64 + cl;
+    const int64_t first = M * blockIdx.y / ST_SPLIT, last = M * (blockIdx.y + 1) / ST_SPLIT;
+    double a = 0.0, q = 0.0;
+    if (c < C) {
+#pragma unroll 8
+        for (int64_t m = first + row; m < last; m += ST_ROWS) {
+            const double v = y[m * ld + c];
+            a += v;
+            q = __builtin_fma(v, v, q);
+        }
+    }
+    red[0][row][cl] = a;
+    red[1][row][cl] = q;
+    __syncthreads();
+    if (row >= 2 || c >= C) return;
+    double t = red[row][0][cl];
+#pragma unroll
+    for (int k = 1; k < ST_ROWS; ++k) t += red[row][k][cl];
+    float* to = acc + (size_t)(2 * blockIdx.y) * 2 * C + row * C + c;
+    const float hi = (float)t;
+    atomicAdd(to, hi);
+    atomicAdd(to + 2 * C, (float)(t - (double)hi));
+}
+int stats_f32(const float* y, int64_t ld, int C, int64_t M, float* acc, hipStream_t s) {
+    hipLaunchKernelGGL(stats_f32_kernel, dim3((C + 63) / 64, ST_SPLIT), dim3(64 * ST_ROWS), 0, s, y, ld, C, M, acc);
+    DS_LAUNCH_CHECK("statistics(fp32)");
+    return 0;
 }
 
 __global__ __launch_bounds__(256) void bn_act_f32_kernel(const dsaspp_bnact_desc d, const int cg, const int64_t total) {
@@ -296,7 +321,6 @@ __global__ __launch_bounds__(256) void bn_act_f32_kernel(const dsaspp_bnact_desc
         }
         v.x = act_clamp(v.x, d.relu); v.y = act_clamp(v.y, d.relu); v.z = act_clamp(v.z, d.relu); v.w = act_clamp(v.w, d.relu);
         *reinterpret_cast<float4*>(yg + m * d.ldy + c) = v;
-        if (d.stat_acc) stat_add4(d.stat_acc, d.C, (int)(m % DS_R), c, v);
     }
 }
 
@@ -318,7 +342,6 @@ __global__ __launch_bounds__(256) void avgpool_f32_kernel(const dsaspp_pool_desc
         const float4 o = make_float4(0.25f * ((a.x + b.x) + (e.x + f.x)), 0.25f * ((a.y + b.y) + (e.y + f.y)),
                                      0.25f * ((a.z + b.z) + (e.z + f.z)), 0.25f * ((a.w + b.w) + (e.w + f.w)));
         *reinterpret_cast<float4*>(yg + m * d.ldy + c) = o;
-        if (d.stat_acc) stat_add4(d.stat_acc, d.C, (int)(m % DS_R), c, o);
     }
 }
 
@@ -386,7 +409,6 @@ __global__ __launch_bounds__(256) void maxpool_f32_kernel(const dsaspp_maxpool_d
 #pragma unroll
             for (int e = 0; e < 4; ++e) d.argmax[m * d.C + c + e] = (uint8_t)pos[e];
         }
-        if (d.stat_acc) stat_add4(d.stat_acc, d.C, (int)(m % DS_R), c, o);
     }
 }
 
@@ -644,7 +666,7 @@ static int conv_f32_one(const dsaspp_conv_desc& d, hipStream_t s) {
     const int nP = (M + FP - 1) / FP, nQ = (d.cout + FQ - 1) / FQ;
     hipLaunchKernelGGL(conv_f32_kernel, dim3(nP * nQ), dim3(256), 0, s, d, M, nQ);
     DS_LAUNCH_CHECK("conv_fwd(fp32)");
-    return 0;
+    return d.stat_acc && !d.g && !d.s_acc ? stats_f32(reinterpret_cast<const float*>(d.y), d.ldy, d.cout, M, d.stat_acc, s) : 0;
 }
 
 int dsaspp_f32_conv(const dsaspp_conv_desc& d, hipStream_t s) {
@@ -740,7 +762,7 @@ int dsaspp_f32_bn_act(const dsaspp_bnact_desc& d, hipStream_t s) {
     const int64_t total = d.M * cg;
     hipLaunchKernelGGL(bn_act_f32_kernel, dim3(blocks_for(total)), dim3(256), 0, s, d, cg, total);
     DS_LAUNCH_CHECK("bn_act(fp32)");
-    return 0;
+    return d.stat_acc ? stats_f32(reinterpret_cast<const float*>(d.y), d.ldy, d.C, d.M, d.stat_acc, s) : 0;
 }
 
 int dsaspp_f32_avgpool(const dsaspp_pool_desc& d, hipStream_t s) {
@@ -748,7 +770,7 @@ int dsaspp_f32_avgpool(const dsaspp_pool_desc& d, hipStream_t s) {
     const int64_t total = (int64_t)d.n_img * (d.H / 2) * (d.W / 2) * cg;
     hipLaunchKernelGGL(avgpool_f32_kernel, dim3(blocks_for(total)), dim3(256), 0, s, d, cg, total);
     DS_LAUNCH_CHECK("avgpool2_fwd(fp32)");
-    return 0;
+    return d.stat_acc ? stats_f32(reinterpret_cast<const float*>(d.y), d.ldy, d.C, total / cg, d.stat_acc, s) : 0;
 }
 
 int dsaspp_f32_im2col(const dsaspp_im2col_desc& d, hipStream_t s) {
@@ -763,7 +785,7 @@ int dsaspp_f32_maxpool(const dsaspp_maxpool_desc& d, hipStream_t s) {
     const int64_t total = (int64_t)d.n_img * (d.H / 2) * (d.W / 2) * cg;
     hipLaunchKernelGGL(maxpool_f32_kernel, dim3(blocks_for(total)), dim3(256), 0, s, d, cg, total);
     DS_LAUNCH_CHECK("maxpool3s2_fwd(fp32)");
-    return 0;
+    return d.stat_acc ? stats_f32(reinterpret_cast<const float*>(d.y), d.ldy, d.C, total / cg, d.stat_acc, s) : 0;
 }
 
 int dsaspp_f32_stem3(const dsaspp_stem3_desc& d, hipStream_t s) {

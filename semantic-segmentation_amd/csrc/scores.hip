@@ -701,16 +701,25 @@ int check(const dsaspp_scores_desc* d, const char* who, Args* a) {
 unsigned grid_for(int64_t blocks) { return (unsigned)(blocks < (1 << 20) ? blocks : (1 << 20)); }
 
 // Pixels per lane, 4 or 1, where the pixels are contiguous.  Forward and 19 classes of 4.2 M pixels, 1 against 4: without alternatives
-// 88 and 85 us (fp32), 68 and 56 (bf16); with one 98 and 104, 88 and 76; with three 113 and 130, 107 and 112; with eight 163 and 207, 172 and 247:
-// four lists of alternatives leave too few waves.  And 4 need enough pixels: 1 M of 150 classes without alternatives 136 and 122 us (fp32), but 94
-// and 113 (bf16, whose loads are half as wide).
+// 84 and 82 us (fp32), 48 and 47 (bf16); with one and what the backward pass needs 98 and 104, 88 and 76; with three 113 and 130, 107 and 112;
+// with eight 163 and 207, 172 and 247: four lists of alternatives leave too few waves.  And 4 need enough pixels, us with 1 and with 4 without alternatives:
+//              9 classes        19             60              150
+//   fp32   1 M  13.8  12.5    20.5  18.8    50.0  44.2    132   121
+//          2 M  23.6  20.9    36.5  33.9     112   120    245   261
+//          4 M  39.5  35.8    84.2  81.6     208   222    467   524
+//   bf16   1 M  10.7  10.1    15.3  16.6    30.5  35.1    80.8  104
+//          2 M  18.2  19.1    26.5  28.2    64.2  76.3    161   202
+//          4 M  32.2  30.1    47.5  46.6     135   141    311   330
+// so many classes take 4 only in fp32 and below 2 M.
 //
 // Backward, 19 classes, one to three alternatives: 262144 pixels 16 against 18 us (fp32) and 10 against 13 (bf16), 400000 pixels 25 and 21, 19 and
-// 16, 4.2 M 261 and 184, 180 and 97: writes of 16 or 8 bytes per lane.  8 pixels of a 16-bit type per lane were slower at every top_k.
+// 16, 4.2 M 261 and 184, 180 and 97: writes of 16 or 8 bytes per lane; 150 classes of 4.2 M 1217 and 1156 (fp32), 1034 and 569 (bf16).  8 pixels of a
+// 16-bit type per lane were slower at every top_k.
 template <int DT, int K, bool BWD>
 int px_per_lane(const Args& a) {
     const int64_t least = BWD ? 3 << 17 : DT == 1 ? 1 << 20 : 1 << 21;
-    return a.d.s2 == 1 && a.d.d2 >= 4 && (BWD || K <= 1) && a.rows >= least ? 4 : 1;
+    const bool many = !BWD && a.d.n_class > 32 && (DT != 1 || a.rows >= 1 << 21);
+    return a.d.s2 == 1 && a.d.d2 >= 4 && (BWD || K <= 1) && a.rows >= least && !many ? 4 : 1;
 }
 
 template <int DT, int K, bool BWD>

@@ -568,6 +568,7 @@ int dsaspp_preprocess(const dsaspp_prep_desc* d, dsaspp_stream_t stream);
  * Rows are numbered (i0, i1, i2) row-major over [d0][d1][d2]; logits of row (i0, i1, i2), class c at
  * logits[i0*s0 + i1*s1 + i2*s2 + c*sc] (strides in elements, >= 0).  labels, logp and entropy are dense [rows];
  * top_logp and top_class are [d0][top_k][d1][d2].  dlogits is dense: [rows][n_class] when sc == 1, else [d0][n_class][d1][d2].
+ * With sc != 1 a lane walks the classes of a row, which is made for many rows of few classes (few rows of many: milliseconds; copy them first).
  * Arithmetic is fp32 on logits of any dtype; dlogits has the logits' dtype (0 = bf16, 1 = fp32, 2 = fp16), rounded once, and must not
  * overlap the logits. */
 #define DSASPP_SCORES_MAX_TOP 8

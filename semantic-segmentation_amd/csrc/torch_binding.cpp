@@ -247,6 +247,7 @@ Out scores_forward(const Plan& p, const Tensor& given, bool need_stats) {
 // An upstream gradient for the kernels: dense, or one value for all (what sum() and mean() send back).
 Tensor upstream(const Tensor& g, const float*& at, int32_t& one) {
     if (!g.defined()) return g;
+    no_tangent(g, "the backward pass of label_scores");
     Tensor t = (g.scalar_type() == at::kFloat ? g : g.to(at::kFloat)).resolve_neg();
     one = 1;
     for (int64_t i = 0; i < t.dim(); ++i)

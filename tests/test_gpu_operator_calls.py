@@ -5,6 +5,7 @@ import time
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwad
 
 import scores_ref as R
 from test_gpu_scores import _tiny
@@ -142,3 +143,16 @@ def test_capture_of_a_network_pass_is_refused(monkeypatch):
         with pytest.raises(RuntimeError, match='captured'):
             mod.score(x)
     assert bool(torch.isfinite(mod.score(x).entropy).all())
+
+
+@pytest.mark.parametrize('upsample,shape', [(1, (6, 19)), (8, (1, 19, 2, 3))])
+def test_dual_upstream_gradients_are_refused(upsample, shape):
+    """Forward mode over the backward pass: its result would lose the tangent."""
+    from test_gpu_scores import _label_scores
+    logits = torch.randn(shape, device='cuda', requires_grad=True)
+    s = _label_scores(logits, upsample=upsample)
+    g = torch.ones_like(s.entropy)
+    with fwad.dual_level():
+        with pytest.raises(RuntimeError, match='forward-mode'):
+            torch.autograd.grad(s.entropy, logits, fwad.make_dual(g, g), retain_graph=True)
+    torch.autograd.grad(s.entropy, logits, g)

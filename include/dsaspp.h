@@ -596,7 +596,8 @@ int dsaspp_scores_bwd(const dsaspp_scores_desc* d, dsaspp_stream_t stream);
 /* The same on logits at 1/8 resolution, with the bilinear x8 upsample (align_corners=False) fused in: the full-resolution logits
  * are never written.  z = hy*r0 + ly*r1, r_i = hx*L[yi][x0] + lx*L[yi][x1], every product and sum rounded to fp32 by itself, so the
  * order of the classes is that of those values to the bit.  What is computed from them has the errors of an fp32 log-softmax, and in pixels
- * whose largest logit is M < 64 in magnitude up to 2 (2 M + 34) half-steps (2^-24) more in a log probability.  A NaN or infinity counts in every pixel whose four source pixels hold it, at weight 0 too, as in torch's upsample.
+ * whose largest logit is M < 64 in magnitude up to 4 M + 92 + 5 (|log p| + entropy) half-steps (2^-24) more in a log probability.  A NaN or
+ * infinity counts in every pixel whose four source pixels hold it, at weight 0 too, as in torch's upsample.
  * n_class <= 32, fewer than 2^24 tiles of 64 x 32 pixels.  Logits of image n, pixel (y, x), class c at
  * logits[n*sn + y*sy + x*sx + c*sc]; labels, logp, entropy [n_img][8h][8w]; top_* [n_img][top_k][8h][8w]; upstream gradients
  * likewise.  Backward reads logits, labels, stats and (with g_entropy) entropy and (with g_top) top_class; dlogits at dlogits[n*gn + y*gy + x*gx + c*gc], dtype g_dtype;

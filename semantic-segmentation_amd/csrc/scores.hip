@@ -8,9 +8,9 @@
 // contiguous: a group of lanes shares a row and reads 16 bytes per lane) and "planes" (class stride other than 1, NCHW: a lane owns
 // P neighbouring pixels and walks the classes).
 //
-// Measured: 4.2 M pixels of 19 fp32 planes with 3 alternatives 114 us (537 MB, 4.7 TB/s); 2.4 M pixels of 19 bf16 planes forward and
-// backward 56 + 58 us (450 MB); 223729 rows of 150 bf16 classes with 3 alternatives 28.5 us (79 MB; vector instructions, 11 of some 20 per
-// class keep the alternatives in order); 8191 rows of 1203 fp32 classes 12 + 18 us.
+// Measured (kernel times): 4.2 M pixels of 19 fp32 planes with 3 alternatives 118 us (537 MB, 4.6 TB/s); 2.4 M pixels of 19 bf16 planes forward
+// and backward 58 + 60 us (450 MB; the forward pass, with half the bytes in flight per load, 3.0 TB/s); 223729 rows of 150 bf16 classes with 3
+// alternatives 32 us (79 MB; vector instructions, 11 of some 20 per class keep the alternatives in order); 8191 rows of 1203 fp32 classes 12 + 18 us.
 #include "softrow.h"
 
 namespace {

@@ -10,8 +10,8 @@
 // pass, which joins no lanes, its 64 columns begin at a multiple of 64 instead (10 x 5 corner pixels), so that a wave writes whole
 // lines: 131 us against 144 at four pictures of 1024 x 2048, 19 classes, 3 alternatives.
 //
-// Measured there: 131 us, 446 MB, 3.4 TB/s.  Training with an entropy term, eight such pictures: 107 us forward (340 MB), 160 backward (400 MB)
-// and 22 for the joining kernel; the vector units are busy 72 % and 85 % of the time.
+// Measured there: 134 us, 446 MB, 3.3 TB/s.  Training with an entropy term, eight such pictures: 110 us forward (340 MB), 163 backward (400 MB)
+// and 22 for the joining kernel; the vector units are busy 71 % and 85 % of the time.
 // The backward pass leaves the sums of every block's 9 x 5 corner pixels in a workspace and a second kernel adds the one to four
 // blocks that meet in a pixel (more on the border) in a fixed order: no atomics, equal inputs give equal bits.
 #include "softrow.h"
@@ -180,7 +180,8 @@ struct Column {
 // What the two forms round differently is z along y (2 half-steps of hy |r0| + ly |r1|) and x (subtraction, scaling, dx, x: 3 of the distance
 // from the maximum and one of dx).  With M = max |M_i| and a class X below the maximum that is 2 (X + M) + 3 X + 34 half-steps in its logit:
 // it falls out of the classes that count, but grows with M.  So columns with M from 64 on take the plain form, which has the errors of an
-// fp32 log-softmax of z; below that a log probability is off by at most 2 (2 M + 34) half-steps more, 2e-5 at M = 64, 6e-6 at M = 10.
+// fp32 log-softmax of z; below that a log probability, which has two such terms and the 23 half-steps of the exponentials, is off by up to
+// 4 M + 92 + 5 (|log p| + H) half-steps more: for likely classes 2e-5 at M = 64, 8e-6 at M = 10.
 // (With M up to 1e5, logits 3 units apart and 1e4 off zero had log probabilities 2e-3 off.)
 // Blocks with logits beyond 1e5, and those with -inf or NaN, take the plain form too: four pictures of 1024 x 2048, 19 classes, 3 alternatives
 // 267 us against 137, forward and backward pass of eight 843 against 270.
@@ -679,7 +680,9 @@ void launch_bwd(const dsaspp_scores8_desc& d, int tx, int ty, unsigned grid, hip
 }  // namespace
 
 // Cityscapes' 19 classes have their own instantiation, every other count the next multiple of 8: the class loops are unrolled
-// registers, and the range checks of the inexact ones cost a select per class.
+// registers, and the range checks of the inexact ones cost a select per class.  Four pictures with 3 alternatives, and forward and backward pass of
+// eight (us):  5 classes 108, 183;  16: 117, 259;  19: 130, 272;  20 to 24: 138, 359;  25 to 32: 176, 616.  The last is LDS: the backward pass keeps
+// two sums per class and lane there, 88 KB in all at 32 classes, so that a CU has one block (three at 19 classes).
 #define BY_CLASSES(F)                                        \
     if (d->n_class == 19) F(19, true);                       \
     else if (d->n_class <= 8) F(8, false);                   \

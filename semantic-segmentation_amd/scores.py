@@ -36,9 +36,9 @@ def label_scores(logits, labels=None, top_k=0, ignore_index=-100, entropy=True, 
     with log probability -inf.  A row with every class masked out has logp -inf (if labelled), entropy 0 and gradient 0.  A NaN or
     +inf in a row makes its logp (if labelled), entropy and top_logp NaN and its top_class -1.  Rows whose upstream gradients
     are all 0 get gradient 0 whatever they hold.  With upsample=8, -inf meets interpolation weights of 0 as in torch's upsample (NaN):
-    give finite logits there.  Its fast form is for pixels whose largest logit is below 64 in magnitude and whose neighbours in the
-    low-resolution picture are no more than 33 units off in any class, all logits below 1e5 in magnitude; the others (a class masked by
-    -1e9, a common offset of 100) cost twice as much, with the backward pass three times, per group of 8 x 4 low-resolution pixels.
+    give finite logits there.  Its fast form takes pixels whose largest logit is below 64 in magnitude, if no class changes its distance from
+    the largest by more than 33 between two low-resolution rows and all logits are below 1e5 in magnitude.  Others (a class masked by -1e9, a
+    common offset of 100) cost twice as much, with the backward pass three times, along with the pixels around them.
 
     logp, entropy and top_logp are differentiable with respect to the logits (once, in reverse mode; dual tensors of forward mode are refused);
     the gradient has the logits' type."""

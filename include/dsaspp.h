@@ -197,6 +197,7 @@ typedef struct dsaspp_bn_desc {
     int32_t use_running;
     float* scale;             /* [C] out (may be NULL) */
     float* shift;
+    int32_t dtype;            /* form of the sums in acc: 0 = bf16 (default), added up in fp32; 1 = fp32, added up in 64 bits */
 } dsaspp_bn_desc;
 
 int dsaspp_bn_finalize(const dsaspp_bn_desc* d, dsaspp_stream_t stream);

@@ -23,17 +23,20 @@ __global__ void bn_finalize_kernel(const dsaspp_bn_desc d) {
     } else {
         const int a = c - d.acc_c0;
         if (d.acc && a >= 0 && a < d.acc_cn) {
-            double s = 0.0, q = 0.0;      // the difference below cancels, and the fp32 form keeps its sums in pairs
-            for (int r = 0; r < DS_R; ++r) {
-                float* row = d.acc + (size_t)r * 2 * d.acc_cn;
-                s += row[a];
-                q += row[d.acc_cn + a];
-                row[a] = 0.f;
-                row[d.acc_cn + a] = 0.f;
-            }
-            const double m = s / d.count;
-            mean = (float)m;
-            var = fmaxf((float)(q / d.count - m * m), 0.f);
+            auto batch = [&](auto zero) {
+                auto s = zero, q = zero;
+                for (int r = 0; r < DS_R; ++r) {
+                    float* row = d.acc + (size_t)r * 2 * d.acc_cn;
+                    s += row[a];
+                    q += row[d.acc_cn + a];
+                    row[a] = 0.f;
+                    row[d.acc_cn + a] = 0.f;
+                }
+                const auto m = s / d.count;
+                mean = (float)m;
+                var = fmaxf((float)(q / d.count - m * m), 0.f);
+            };
+            if (d.dtype == 1) batch(0.0); else batch(0.f);      // the fp32 form keeps its sums in pairs, and the difference cancels
             d.mean[c] = mean;
             d.var[c] = var;
             d.rstd[c] = rsqrtf(var + d.eps);

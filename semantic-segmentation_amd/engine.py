@@ -40,7 +40,7 @@ class Ref:
 
 # ops whose descriptor carries the activation storage type (include/dsaspp.h: `dtype`)
 _DTYPE_OPS = frozenset(('conv', 'bn_act', 'avgpool_fwd', 'im2col', 'maxpool_fwd', 'stem3', 'dwconv', 'wgrad', 'grad_extract',
-                        'bn_bwd_apply', 'avgpool_bwd', 'maxpool_bwd', 'col2im'))
+                        'bn_bwd_apply', 'avgpool_bwd', 'maxpool_bwd', 'col2im', 'bn_finalize'))
 
 
 class OpList(list):

@@ -121,6 +121,9 @@ c10::intrusive_ptr<Plan> make_plan(at::IntArrayRef shape, at::Device device, con
     p->c = shape[1];
     VALUE_CHECK(p->c >= 1 && p->c < (1 << 30) && (!up || p->c <= MAX_CLASSES_UPSAMPLED), "%lld classes: at least one%s", (long long)p->c,
                 up ? ", at most 32 with upsample=8" : "");
+    // before the narrowing to the descriptor's 32 bits, which would make another picture of it
+    VALUE_CHECK(!up || (p->n < (1ll << 31) && shape[2] < (1 << 20) && shape[3] < (1 << 20)), "logits of shape %s are too large for upsample=8: pictures below 2^20 x 2^20, "
+                "fewer than 2^31", shape_text(shape).c_str());
     VALUE_CHECK(top_k >= 0 && top_k <= std::min<int64_t>(DSASPP_SCORES_MAX_TOP, p->c), "top_k must be in [0, %d] and at most the %lld classes, got %lld",
                 DSASPP_SCORES_MAX_TOP, (long long)p->c, (long long)top_k);
     VALUE_CHECK(labels.has_value() || entropy || top_k, "nothing to compute: no labels, no entropy, top_k = 0");

@@ -108,3 +108,11 @@ def test_a_refused_update_leaves_the_optimizer_as_it_was(monkeypatch):
     monkeypatch.setattr(optim, 'adam_update_', lambda p, g, m, v, step, **k: torch.tensor(float(step) * k['grad_scale']))
     assert float(opt.step(max_grad_norm=1.0)) == 0.25
     assert opt.step_count == 1 and mod._grad_scale == 1.0
+
+
+def test_sizes_beyond_32_bits_are_refused_before_they_are_narrowed():
+    check = _lib.binding().check_scores
+    for shape in ([1, 19, 4, 2 ** 32 + 5], [1, 19, 2 ** 32 + 5, 4], [2 ** 32 + 1, 2, 1, 1], [1, 19, 1 << 20, 4]):
+        with pytest.raises(ValueError, match='too large'):
+            check(shape, 'cuda:0', None, 0, True, 8)
+    check([1, 19, (1 << 20) - 1, 4], 'cuda:0', None, 0, True, 8)
